@@ -897,6 +897,66 @@ int ssc_field_scale_f32(const float *x /* [n,c] */, int64_t n, int32_t c,
                         const int32_t *field_of /* [c] */, float *y /* [n,c] */,
                         ssc_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Operators of pointwise training blocks on rows [n, c] (no counterpart in the reference,
+ * whose blocks are convolution, batch norm and gate).  Arrays named `void *` hold elements of
+ * the type `dtype` says; sums and statistics are held in 32 bits or more and every result is
+ * rounded once.
+ * ---------------------------------------------------------------------- */
+#define SSC_F32 0
+#define SSC_F16 1
+#define SSC_BF16 2
+
+/* Activations of these operators, beside SSC_ACT_NONE .. SSC_ACT_TANH. */
+#define SSC_ACT_SILU 4 /* z / (1 + exp(-z)) */
+#define SSC_ACT_GELU 5 /* z (1 + erf(z / sqrt 2)) / 2 */
+
+/* Group norm with an activation.  The rows of cloud b are offsets[b] .. offsets[b + 1] - 1
+ * (ascending; the first cloud begins at row 0 and the last ends at row n whatever offsets[0] and
+ * offsets[clouds] hold; clouds may be empty); group g holds channels g c / groups ...
+ *   z = weight (x - mean) / sqrt(var + eps) + bias,  y = act(z)
+ * with the mean and the (biased) variance of a cloud's group.  weight, bias [c] of type wtype, or
+ * NULL (1 and 0).  mean, rstd [clouds, groups] are written for the backward pass (0 for empty
+ * clouds).  ssc_groupnorm_bwd: dx [n,c], dweight, dbias [c] of type wtype, each NULL where it is
+ * not wanted.  With n = 0 nothing is written. */
+size_t ssc_groupnorm_workspace_bytes(int64_t n, int32_t c, int32_t clouds, int32_t groups);
+int ssc_groupnorm_fwd(int32_t dtype, const void *x /* [n,c] */, int64_t n, int32_t c,
+                      const int32_t *offsets /* [clouds + 1] */, int32_t clouds, int32_t groups,
+                      int32_t wtype, const void *weight, const void *bias, float eps, int32_t act,
+                      void *y /* [n,c] */, float *mean, float *rstd, void *workspace,
+                      size_t workspace_bytes, ssc_stream_t stream);
+int ssc_groupnorm_bwd(int32_t dtype, const void *x, const void *dy /* [n,c] */, int64_t n, int32_t c,
+                      const int32_t *offsets, int32_t clouds, int32_t groups, int32_t wtype,
+                      const void *weight, const void *bias, int32_t act, const float *mean,
+                      const float *rstd, void *dx, void *dweight, void *dbias, void *workspace,
+                      size_t workspace_bytes, ssc_stream_t stream);
+
+/* One AdamW step over n_tensors tensors (host array), each updated in place:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * state_bits 32: exp_avg, exp_avg_sq are floats.  state_bits 8: exp_avg is int8_t and exp_avg_sq
+ * uint8_t with one float scale q for each SSC_ADAMW_BLOCK elements (the last block may be
+ * shorter): m = q c |c|, sqrt(v) = q c^2.  param and grad are of type dtype, aligned to their
+ * elements; 16 bytes (codes: 4) make it faster.  No two tensors may overlap.
+ * ssc_adamw_values writes what 8-bit moments stand for: m to `param`, v to `grad` (float arrays;
+ * either may be NULL), dtype SSC_F32. */
+#define SSC_ADAMW_BLOCK 256
+typedef struct ssc_adamw_tensor {
+  void *param;
+  void *grad;
+  void *exp_avg;
+  void *exp_avg_sq;
+  float *exp_avg_scale;    /* state_bits 8 */
+  float *exp_avg_sq_scale; /* state_bits 8 */
+  int64_t numel;
+  int64_t dtype;
+} ssc_adamw_tensor;
+int ssc_adamw_step(const ssc_adamw_tensor *tensors /* host */, int32_t n_tensors,
+                   int32_t state_bits, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, int64_t step, ssc_stream_t stream);
+int ssc_adamw_values(const ssc_adamw_tensor *tensors /* host */, int32_t n_tensors,
+                     ssc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

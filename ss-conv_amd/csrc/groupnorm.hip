@@ -1,0 +1,627 @@
+// Group norm with an activation over rows [n, c], channels last, rows grouped by cloud.
+//
+// Cloud b, group g (c / groups neighbouring channels), m = rows(b) * c / groups values:
+//   mean, var = E[(x - mean)^2], rstd = 1 / sqrt(var + eps), h = (x - mean) rstd,
+//   z = weight h + bias, y = f(z)
+// and with dz = dy f'(z)
+//   dbias = sum dz, dweight = sum dz h, S1 = sum over the group of weight dz, S2 = of weight dz h
+//   dx = rstd (weight dz - (S1 + h S2) / m).
+//
+// HBM-bound: x has to be read before the first y can be written, so a pass takes the sums and
+// another one applies them.  Rows are cut into chunks of equal length whatever the clouds are; a
+// chunk that spans a boundary holds one piece of each cloud, and the partial result of cloud b's
+// piece in chunk k goes to slot k + b: along the rows each next piece moves k or b by at least
+// one, so no two pieces share a slot and no table of pieces is needed.
+//
+// The variance comes from deviations, not from E[x^2] - mean^2: a thread sums x - x0 and
+// (x - x0)^2 with its own first value x0 of the channel, which leaves numbers of the spread's
+// size, and partial results (count, mean, sum of squared deviations) are joined by
+// M = M1 + M2 + (mean2 - mean1)^2 n1 n2 / (n1 + n2).  Every order is fixed: results are
+// reproducible.
+#include "elem.h"
+
+namespace ssc {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kChunksMost = 2048;  // chunks of rows: eight workgroups for each of 256 CUs
+
+struct Norm {
+  const void *x, *dy;
+  void *out;                 // y or dx
+  const int32_t *offsets;    // [clouds + 1]
+  const void *weight, *bias;  // [c] or NULL
+  float *mean, *rstd;        // [clouds, groups]
+  float2 *partial;           // [chunks + clouds, c]
+  float2 *sums;              // [clouds, c]: sum dz, sum dz h
+  float2 *group;             // [clouds, groups]: S1 / m, S2 / m
+  void *dweight, *dbias;     // [c] or NULL
+  int64_t n;
+  int32_t c, clouds, groups, per, wtype, act, rows;  // rows: of a chunk
+  float eps;
+};
+
+// Rows of cloud b: they begin at 0 and end at n whatever the first and last offset say, and
+// never lie outside the rows.
+__device__ __forceinline__ int64_t cloud_begin(const Norm &a, int b) {
+  if (b <= 0) return 0;
+  if (b >= a.clouds) return a.n;
+  const int64_t o = a.offsets[b];
+  return o < 0 ? 0 : o > a.n ? a.n : o;
+}
+
+// The first cloud that ends behind row r.
+__device__ __forceinline__ int cloud_of(const Norm &a, int64_t r) {
+  int lo = 0, hi = a.clouds - 1;  // the answer is in lo .. hi
+  while (hi - lo > 63) {
+    const int mid = (lo + hi) >> 1;
+    if (cloud_begin(a, mid + 1) > r) hi = mid;
+    else lo = mid + 1;
+  }
+  const int i = lo + (int)(threadIdx.x & 63);
+  const int below = __popcll(__ballot(i < hi && cloud_begin(a, i + 1) <= r));
+  return __builtin_amdgcn_readfirstlane(lo + below);
+}
+
+// How the threads of a workgroup lie on rows and channels: `tx` threads of V channels side by
+// side, `ty` rows at a time, column tile blockIdx.y.
+template <int V> struct Lay {
+  int tx, ty, cx, row;
+  int64_t ch;
+  bool in;
+  __device__ Lay(const Norm &a) {
+    const int cv = a.c / V;
+    tx = cv < kThreads ? cv : kThreads;
+    ty = kThreads / tx;
+    row = (int)threadIdx.x / tx;
+    cx = (int)threadIdx.x - row * tx;
+    ch = ((int64_t)blockIdx.y * tx + cx) * V;
+    in = row < ty && ch < a.c;
+  }
+};
+
+constexpr int kUnroll = 4;  // rows of a thread whose loads are in flight together
+
+// ---- statistics ---------------------------------------------------------------------------
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) norm_stats_kernel(const Norm a) {
+  __shared__ float2 lds[kThreads * V];
+  __shared__ float counts[kThreads];
+  const Lay<V> lay(a);
+  const int64_t r0 = (int64_t)blockIdx.x * a.rows;
+  const int64_t r1 = r0 + a.rows < a.n ? r0 + a.rows : a.n;
+  const T *x = static_cast<const T *>(a.x) + lay.ch;
+  for (int b = cloud_of(a, r0); b < a.clouds; ++b) {
+    const int64_t cb = cloud_begin(a, b), ce = cloud_begin(a, b + 1);
+    if (cb >= r1) break;
+    const int64_t s = cb > r0 ? cb : r0, e = ce < r1 ? ce : r1;
+    if (s >= e) continue;
+    float first[V], s1[V], s2[V], count = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) first[i] = s1[i] = s2[i] = 0.f;
+    if (lay.in && s + lay.row < e) {
+      int64_t r = s + lay.row;
+      load_floats<T, V>(x + r * a.c, first);
+      for (; r + (kUnroll - 1) * lay.ty < e; r += kUnroll * lay.ty) {
+        float v[kUnroll][V];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) load_floats<T, V>(x + (r + u * lay.ty) * a.c, v[u]);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float d = v[u][i] - first[i];
+            s1[i] += d;
+            s2[i] += d * d;
+          }
+        count += kUnroll;
+      }
+      for (; r < e; r += lay.ty) {
+        float v[V];
+        load_floats<T, V>(x + r * a.c, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = v[i] - first[i];
+          s1[i] += d;
+          s2[i] += d * d;
+        }
+        count += 1.f;
+      }
+    }
+    const float inv = count > 0.f ? 1.f / count : 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float d = s1[i] * inv;
+      lds[threadIdx.x * V + i] = make_float2(first[i] + d, fmaxf(s2[i] - s1[i] * d, 0.f));
+    }
+    counts[threadIdx.x] = count;
+    __syncthreads();
+    int half = 1;
+    while (half * 2 < lay.ty) half *= 2;
+    for (; half > 0 && lay.ty > 1; half >>= 1) {
+      if (lay.row < half && lay.row + half < lay.ty) {
+        const int o = threadIdx.x + half * lay.tx;
+        const float n1 = counts[threadIdx.x], n2 = counts[o];
+        if (n2 > 0.f) {  // (rows are dealt in order: n1 >= n2)
+          const float w2 = n2 / (n1 + n2), w = n1 * w2;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float2 p = lds[threadIdx.x * V + i], q = lds[o * V + i];
+            const float d = q.x - p.x;
+            lds[threadIdx.x * V + i] = make_float2(p.x + d * w2, p.y + q.y + d * d * w);
+          }
+        }
+      }
+      __syncthreads();
+      if (lay.row < half && lay.row + half < lay.ty && lay.cx < lay.tx)
+        counts[threadIdx.x] += counts[threadIdx.x + half * lay.tx];
+      __syncthreads();
+    }
+    if (lay.in && lay.row == 0) {
+      float2 *p = a.partial + ((int64_t)blockIdx.x + b) * a.c + lay.ch;
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[i] = lds[threadIdx.x * V + i];
+    }
+    __syncthreads();
+  }
+}
+
+// Sum over the workgroup, the same in every thread.
+template <typename S>
+__device__ __forceinline__ S block_sum(S v, S *lds) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  S t = 0;
+  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) t += lds[w];
+  return t;
+}
+
+// mean and rstd of group blockIdx.x % groups of cloud blockIdx.x / groups, from the channels'
+// means and squared deviations in the pieces of the cloud.  Sums over at most a few thousand
+// numbers, in double: their cost does not show.
+__global__ void __launch_bounds__(1024) norm_finish_kernel(const Norm a) {
+  __shared__ double lds[16];
+  const int b = blockIdx.x / a.groups, g = blockIdx.x - b * a.groups;
+  const int64_t s = cloud_begin(a, b), e = cloud_begin(a, b + 1);
+  if (s >= e) {
+    if (threadIdx.x == 0) {
+      a.mean[blockIdx.x] = 0.f;
+      a.rstd[blockIdx.x] = 0.f;
+    }
+    return;
+  }
+  const int64_t k0 = s / a.rows, k1 = (e - 1) / a.rows;
+  const float2 *p = a.partial + (k0 + b) * a.c + (int64_t)g * a.per;
+  const double shift = p[0].x;
+  double n = 0, s1 = 0, s2 = 0;
+  const int64_t items = (k1 - k0 + 1) * a.per;
+  for (int64_t i = threadIdx.x; i < items; i += blockDim.x) {
+    const int64_t k = i / a.per;
+    const float2 v = p[k * a.c + (i - k * a.per)];
+    const int64_t kb = (k0 + k) * a.rows, ke = kb + a.rows;
+    const double rows = (double)((ke < e ? ke : e) - (kb > s ? kb : s));
+    const double d = (double)v.x - shift;
+    n += rows;
+    s1 += rows * d;
+    s2 += (double)v.y + rows * d * d;
+  }
+  n = block_sum(n, lds);
+  s1 = block_sum(s1, lds);
+  s2 = block_sum(s2, lds);
+  if (threadIdx.x == 0) {
+    const double d = s1 / n, var = s2 / n - d * d;
+    a.mean[blockIdx.x] = (float)(shift + d);
+    a.rstd[blockIdx.x] = (float)(1.0 / sqrt((var < 0 ? 0 : var) + (double)a.eps));
+  }
+}
+
+// ---- y --------------------------------------------------------------------------------------
+// What the channels of a thread need of cloud b.
+template <int V>
+__device__ __forceinline__ void channel_consts(const Norm &a, int b, int64_t ch, float *mean,
+                                               float *rstd) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int64_t g = (int64_t)b * a.groups + (ch + i) / a.per;
+    mean[i] = a.mean[g];
+    rstd[i] = a.rstd[g];
+  }
+}
+template <int V>
+__device__ __forceinline__ void channel_params(const Norm &a, int64_t ch, float *w, float *bias) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    w[i] = a.weight ? load_any(a.weight, ch + i, a.wtype) : 1.f;
+    bias[i] = a.bias ? load_any(a.bias, ch + i, a.wtype) : 0.f;
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) norm_apply_kernel(const Norm a) {
+  const Lay<V> lay(a);
+  if (!lay.in) return;
+  const int64_t r0 = (int64_t)blockIdx.x * a.rows;
+  const int64_t r1 = r0 + a.rows < a.n ? r0 + a.rows : a.n;
+  const T *x = static_cast<const T *>(a.x) + lay.ch;
+  T *y = static_cast<T *>(a.out) + lay.ch;
+  float w[V], bias[V];
+  channel_params<V>(a, lay.ch, w, bias);
+  for (int b = cloud_of(a, r0); b < a.clouds; ++b) {
+    const int64_t cb = cloud_begin(a, b), ce = cloud_begin(a, b + 1);
+    if (cb >= r1) break;
+    const int64_t s = cb > r0 ? cb : r0, e = ce < r1 ? ce : r1;
+    if (s >= e) continue;
+    float mean[V], rstd[V];
+    channel_consts<V>(a, b, lay.ch, mean, rstd);
+#pragma unroll
+    for (int i = 0; i < V; ++i) rstd[i] *= w[i];
+    for (int64_t r = s + lay.row; r < e; r += lay.ty * kUnroll) {
+      float v[kUnroll][V], z[V];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (r + u * lay.ty < e) load_floats<T, V>(x + (r + u * lay.ty) * a.c, v[u]);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (r + u * lay.ty < e) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) z[i] = (v[u][i] - mean[i]) * rstd[i] + bias[i];
+          activate<V>(a.act, z, v[u]);
+          store_floats<T, V>(y + (r + u * lay.ty) * a.c, v[u]);
+        }
+    }
+  }
+}
+
+// ---- backward -------------------------------------------------------------------------------
+// h and dz of one row's V channels.
+template <int V>
+__device__ __forceinline__ void row_terms(int act, const float *x, const float *dy,
+                                          const float *mean, const float *rstd, const float *w,
+                                          const float *bias, float *h, float *dz) {
+  float z[V], f[V], d[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    h[i] = (x[i] - mean[i]) * rstd[i];
+    z[i] = h[i] * w[i] + bias[i];
+  }
+  activate_slope<V>(act, z, f, d);
+#pragma unroll
+  for (int i = 0; i < V; ++i) dz[i] = dy[i] * d[i];
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) norm_sums_kernel(const Norm a) {
+  __shared__ float2 lds[kThreads * V];
+  const Lay<V> lay(a);
+  const int64_t r0 = (int64_t)blockIdx.x * a.rows;
+  const int64_t r1 = r0 + a.rows < a.n ? r0 + a.rows : a.n;
+  const T *x = static_cast<const T *>(a.x) + lay.ch;
+  const T *dy = static_cast<const T *>(a.dy) + lay.ch;
+  float w[V], bias[V];
+  if (lay.in) channel_params<V>(a, lay.ch, w, bias);
+  for (int b = cloud_of(a, r0); b < a.clouds; ++b) {
+    const int64_t cb = cloud_begin(a, b), ce = cloud_begin(a, b + 1);
+    if (cb >= r1) break;
+    const int64_t s = cb > r0 ? cb : r0, e = ce < r1 ? ce : r1;
+    if (s >= e) continue;
+    float s1[V], s2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+    if (lay.in) {
+      float mean[V], rstd[V];
+      channel_consts<V>(a, b, lay.ch, mean, rstd);
+      for (int64_t r = s + lay.row; r < e; r += lay.ty * kUnroll) {
+        float v[kUnroll][V], g[kUnroll][V];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (r + u * lay.ty < e) {
+            load_floats<T, V>(x + (r + u * lay.ty) * a.c, v[u]);
+            load_floats<T, V>(dy + (r + u * lay.ty) * a.c, g[u]);
+          }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (r + u * lay.ty < e) {
+            float h[V], dz[V];
+            row_terms<V>(a.act, v[u], g[u], mean, rstd, w, bias, h, dz);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              s1[i] += dz[i];
+              s2[i] += dz[i] * h[i];
+            }
+          }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) lds[threadIdx.x * V + i] = make_float2(s1[i], s2[i]);
+    __syncthreads();
+    int half = 1;
+    while (half * 2 < lay.ty) half *= 2;
+    for (; half > 0 && lay.ty > 1; half >>= 1) {
+      if (lay.row < half && lay.row + half < lay.ty) {
+        const int o = threadIdx.x + half * lay.tx;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float2 p = lds[threadIdx.x * V + i], q = lds[o * V + i];
+          lds[threadIdx.x * V + i] = make_float2(p.x + q.x, p.y + q.y);
+        }
+      }
+      __syncthreads();
+    }
+    if (lay.in && lay.row == 0) {
+      float2 *p = a.partial + ((int64_t)blockIdx.x + b) * a.c + lay.ch;
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[i] = lds[threadIdx.x * V + i];
+    }
+    __syncthreads();
+  }
+}
+
+// Group blockIdx.x % groups of cloud blockIdx.x / groups: the pieces' sums added up, channel by
+// channel, and S1 / m, S2 / m of the group.
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(const Norm a) {
+  __shared__ float2 lds[1024];
+  __shared__ float total[16];
+  const int b = blockIdx.x / a.groups, g = blockIdx.x - b * a.groups;
+  const int64_t s = cloud_begin(a, b), e = cloud_begin(a, b + 1);
+  const int64_t k0 = s / a.rows, k1 = s < e ? (e - 1) / a.rows + 1 : k0;
+  const int threads = blockDim.x;
+  float t1 = 0.f, t2 = 0.f;
+  for (int c0 = 0; c0 < a.per; c0 += threads) {  // (one turn unless a group has over 1024 channels)
+    const int tx = a.per - c0 < threads ? a.per - c0 : threads, ty = threads / tx;
+    const int row = threadIdx.x / tx, cx = threadIdx.x - row * tx;
+    const int64_t ch = (int64_t)g * a.per + c0 + cx;
+    float s1 = 0.f, s2 = 0.f;
+    if (row < ty)
+      for (int64_t k = k0 + row; k < k1; k += ty) {
+        const float2 v = a.partial[(k + b) * a.c + ch];
+        s1 += v.x;
+        s2 += v.y;
+      }
+    __syncthreads();
+    lds[threadIdx.x] = make_float2(s1, s2);
+    __syncthreads();
+    if (row == 0) {
+      for (int y = 1; y < ty; ++y) {
+        s1 += lds[y * tx + cx].x;
+        s2 += lds[y * tx + cx].y;
+      }
+      a.sums[(int64_t)b * a.c + ch] = make_float2(s1, s2);
+      const float w = a.weight ? load_any(a.weight, ch, a.wtype) : 1.f;
+      t1 += w * s1;
+      t2 += w * s2;
+    }
+  }
+  t1 = block_sum(t1, total);
+  t2 = block_sum(t2, total);
+  if (threadIdx.x == 0) {
+    const float inv = s < e ? 1.f / ((float)(e - s) * (float)a.per) : 0.f;
+    a.group[blockIdx.x] = make_float2(t1 * inv, t2 * inv);
+  }
+}
+
+// dweight and dbias of 16 channels, from the clouds' sums.
+__device__ __forceinline__ void param_grads(const Norm &a, int block) {
+  __shared__ float2 lds[kThreads];
+  const int cx = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const int64_t ch = (int64_t)block * 16 + cx;
+  float s1 = 0.f, s2 = 0.f;
+  if (ch < a.c)
+    for (int b = row; b < a.clouds; b += kThreads / 16) {
+      const float2 v = a.sums[(int64_t)b * a.c + ch];
+      s1 += v.x;
+      s2 += v.y;
+    }
+  lds[threadIdx.x] = make_float2(s1, s2);
+  __syncthreads();
+  if (row == 0 && ch < a.c) {
+    for (int y = 1; y < kThreads / 16; ++y) {
+      s1 += lds[y * 16 + cx].x;
+      s2 += lds[y * 16 + cx].y;
+    }
+    if (a.dbias) store_any(a.dbias, ch, a.wtype, s1);
+    if (a.dweight) store_any(a.dweight, ch, a.wtype, s2);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) norm_params_kernel(const Norm a) {
+  param_grads(a, blockIdx.x);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) norm_dx_kernel(const Norm a) {
+  const Lay<V> lay(a);
+  if (!lay.in) return;
+  const int64_t r0 = (int64_t)blockIdx.x * a.rows;
+  const int64_t r1 = r0 + a.rows < a.n ? r0 + a.rows : a.n;
+  const T *x = static_cast<const T *>(a.x) + lay.ch;
+  const T *dy = static_cast<const T *>(a.dy) + lay.ch;
+  T *dx = static_cast<T *>(a.out) + lay.ch;
+  float w[V], bias[V];
+  channel_params<V>(a, lay.ch, w, bias);
+  for (int b = cloud_of(a, r0); b < a.clouds; ++b) {
+    const int64_t cb = cloud_begin(a, b), ce = cloud_begin(a, b + 1);
+    if (cb >= r1) break;
+    const int64_t s = cb > r0 ? cb : r0, e = ce < r1 ? ce : r1;
+    if (s >= e) continue;
+    float mean[V], rstd[V], m1[V], m2[V];
+    channel_consts<V>(a, b, lay.ch, mean, rstd);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 v = a.group[(int64_t)b * a.groups + (lay.ch + i) / a.per];
+      m1[i] = v.x;
+      m2[i] = v.y;
+    }
+    for (int64_t r = s + lay.row; r < e; r += lay.ty * kUnroll) {
+      float v[kUnroll][V], g[kUnroll][V];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (r + u * lay.ty < e) {
+          load_floats<T, V>(x + (r + u * lay.ty) * a.c, v[u]);
+          load_floats<T, V>(dy + (r + u * lay.ty) * a.c, g[u]);
+        }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (r + u * lay.ty < e) {
+          float h[V], dz[V];
+          row_terms<V>(a.act, v[u], g[u], mean, rstd, w, bias, h, dz);
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[u][i] = rstd[i] * (w[i] * dz[i] - (m1[i] + h[i] * m2[i]));
+          store_floats<T, V>(dx + (r + u * lay.ty) * a.c, v[u]);
+        }
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------
+// Rows of a chunk: enough that at most kChunksMost chunks are left, and at least 32, so that the
+// partial results stay small beside the rows.
+int64_t chunk_rows(int64_t n) {
+  const int64_t r = ceil_div(n, kChunksMost);
+  return r < 32 ? 32 : r;
+}
+
+bool same_alignment(const void *a, const void *b, const void *c, size_t to) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) |
+           reinterpret_cast<uintptr_t>(c)) & (to - 1)) == 0;
+}
+
+dim3 chunk_grid(const Norm &a, int v) {
+  const int cv = a.c / v;
+  const int tx = cv < kThreads ? cv : kThreads;
+  return dim3((uint32_t)ceil_div(a.n, a.rows), (uint32_t)ceil_div(cv, tx));
+}
+
+// Threads of a workgroup that adds up the pieces of one group.
+int finish_threads(const Norm &a) {
+  const int64_t items = (ceil_div(a.n, a.rows) / a.clouds + 1) * a.per;
+  return items > 2048 ? 1024 : items > 256 ? 256 : 64;
+}
+
+template <typename T> int forward(const Norm &a, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const bool wide = a.c % V == 0 && same_alignment(a.x, a.x, a.out, 16);
+  if (wide) hipLaunchKernelGGL((norm_stats_kernel<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a);
+  else hipLaunchKernelGGL((norm_stats_kernel<T, 1>), chunk_grid(a, 1), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(norm_finish_kernel, dim3(a.clouds * a.groups), dim3(finish_threads(a)), 0, s, a);
+  if (wide) hipLaunchKernelGGL((norm_apply_kernel<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a);
+  else hipLaunchKernelGGL((norm_apply_kernel<T, 1>), chunk_grid(a, 1), dim3(kThreads), 0, s, a);
+  SSC_LAUNCH_CHECK("group norm, forward");
+  return SSC_OK;
+}
+
+template <typename T> int backward(const Norm &a, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const bool wide = a.c % V == 0 && same_alignment(a.x, a.dy, a.out, 16);
+  if (wide) hipLaunchKernelGGL((norm_sums_kernel<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a);
+  else hipLaunchKernelGGL((norm_sums_kernel<T, 1>), chunk_grid(a, 1), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(norm_reduce_kernel, dim3(a.clouds * a.groups), dim3(finish_threads(a)), 0, s, a);
+  if (a.dweight || a.dbias)
+    hipLaunchKernelGGL(norm_params_kernel, dim3((uint32_t)ceil_div(a.c, 16)), dim3(kThreads), 0, s, a);
+  if (a.out && wide) hipLaunchKernelGGL((norm_dx_kernel<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a);
+  else if (a.out) hipLaunchKernelGGL((norm_dx_kernel<T, 1>), chunk_grid(a, 1), dim3(kThreads), 0, s, a);
+  SSC_LAUNCH_CHECK("group norm, backward");
+  return SSC_OK;
+}
+
+size_t workspace(int64_t n, int32_t c, int32_t clouds, int32_t groups) {
+  if (n <= 0) return 256;
+  const int64_t chunks = ceil_div(n, chunk_rows(n));
+  return align_up((size_t)(chunks + clouds) * c * sizeof(float2)) +
+         align_up((size_t)clouds * c * sizeof(float2)) +
+         align_up((size_t)clouds * groups * sizeof(float2));
+}
+
+int check(int32_t dtype, int64_t n, int32_t c, const int32_t *offsets, int32_t clouds,
+          int32_t groups, int32_t wtype, int32_t act, const void *ws, size_t ws_bytes) {
+  SSC_CHECK(dtype_ok(dtype), SSC_EINVAL, "element type %d", dtype);
+  SSC_CHECK(dtype_ok(wtype), SSC_EINVAL, "element type %d of the parameters", wtype);
+  SSC_CHECK(n >= 0 && c >= 1 && groups >= 1 && c % groups == 0, SSC_EINVAL,
+            "%lld rows of %d channels cannot be cut into %d groups", (long long)n, c, groups);
+  SSC_CHECK(n <= 0x7FFFFFFF, SSC_EINVAL, "offsets of rows are int32: %lld rows", (long long)n);
+  SSC_CHECK(clouds >= (n > 0 ? 1 : 0) && (int64_t)clouds * groups <= 0x7FFFFFFF, SSC_EINVAL,
+            "%d clouds of %d groups", clouds, groups);
+  SSC_CHECK(pointwise_act_ok(act), SSC_EINVAL, "activation %d", act);
+  SSC_CHECK(n == 0 || offsets != nullptr, SSC_EINVAL, "offsets is NULL");
+  SSC_CHECK(n == 0 || (ws != nullptr && ws_bytes >= workspace(n, c, clouds, groups)), SSC_EWORKSPACE,
+            "workspace of %zu bytes, %zu are needed", ws_bytes, workspace(n, c, clouds, groups));
+  return SSC_OK;
+}
+
+Norm carve(int64_t n, int32_t c, int32_t clouds, int32_t groups, void *ws) {
+  Norm a = {};
+  a.n = n;
+  a.c = c;
+  a.clouds = clouds;
+  a.groups = groups;
+  a.per = c / groups;
+  a.rows = (int32_t)chunk_rows(n);
+  Carver w(ws);
+  a.partial = w.take<float2>((size_t)(ceil_div(n, a.rows) + clouds) * c);
+  a.sums = w.take<float2>((size_t)clouds * c);
+  a.group = w.take<float2>((size_t)clouds * groups);
+  return a;
+}
+
+}  // namespace
+}  // namespace ssc
+
+using namespace ssc;
+
+extern "C" size_t ssc_groupnorm_workspace_bytes(int64_t n, int32_t c, int32_t clouds,
+                                                int32_t groups) {
+  return workspace(n, c, clouds, groups);
+}
+
+extern "C" int ssc_groupnorm_fwd(int32_t dtype, const void *x, int64_t n, int32_t c,
+                                 const int32_t *offsets, int32_t clouds, int32_t groups,
+                                 int32_t wtype, const void *weight, const void *bias, float eps,
+                                 int32_t act, void *y, float *mean, float *rstd, void *ws,
+                                 size_t ws_bytes, ssc_stream_t stream) {
+  const int rc = check(dtype, n, c, offsets, clouds, groups, wtype, act, ws, ws_bytes);
+  if (rc != SSC_OK) return rc;
+  SSC_CHECK(eps >= 0.f, SSC_EINVAL, "eps is not negative");
+  if (n == 0) return SSC_OK;
+  SSC_CHECK(x && y && mean && rstd, SSC_EINVAL, "NULL pointer");
+  Norm a = carve(n, c, clouds, groups, ws);
+  a.x = x;
+  a.out = y;
+  a.offsets = offsets;
+  a.weight = weight;
+  a.bias = bias;
+  a.wtype = wtype;
+  a.act = act;
+  a.eps = eps;
+  a.mean = mean;
+  a.rstd = rstd;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == SSC_F32 ? forward<float>(a, s) : dtype == SSC_F16 ? forward<f16>(a, s) : forward<bf16>(a, s);
+}
+
+extern "C" int ssc_groupnorm_bwd(int32_t dtype, const void *x, const void *dy, int64_t n, int32_t c,
+                                 const int32_t *offsets, int32_t clouds, int32_t groups,
+                                 int32_t wtype, const void *weight, const void *bias, int32_t act,
+                                 const float *mean, const float *rstd, void *dx, void *dweight,
+                                 void *dbias, void *ws, size_t ws_bytes, ssc_stream_t stream) {
+  const int rc = check(dtype, n, c, offsets, clouds, groups, wtype, act, ws, ws_bytes);
+  if (rc != SSC_OK) return rc;
+  if (n == 0) return SSC_OK;
+  SSC_CHECK(x && dy && mean && rstd, SSC_EINVAL, "NULL pointer");
+  Norm a = carve(n, c, clouds, groups, ws);
+  a.x = x;
+  a.dy = dy;
+  a.out = dx;
+  a.offsets = offsets;
+  a.weight = weight;
+  a.bias = bias;
+  a.wtype = wtype;
+  a.act = act;
+  a.mean = const_cast<float *>(mean);
+  a.rstd = const_cast<float *>(rstd);
+  a.dweight = dweight;
+  a.dbias = dbias;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == SSC_F32 ? backward<float>(a, s) : dtype == SSC_F16 ? backward<f16>(a, s) : backward<bf16>(a, s);
+}

@@ -8,5 +8,8 @@ from . import activation
 from . import batchnorm
 from . import pool
 from . import dropout
+from . import groupnorm
+from . import optim
 
-__all__ = ["sp_ops", "utils", "convolution", "activation", "batchnorm", "pool", "dropout"]
+__all__ = ["sp_ops", "utils", "convolution", "activation", "batchnorm", "pool", "dropout",
+           "groupnorm", "optim"]

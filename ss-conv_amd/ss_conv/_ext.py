@@ -35,6 +35,16 @@ class Geometry(ctypes.Structure):
 
 _gp = ctypes.POINTER(Geometry)
 
+
+class AdamwTensor(ctypes.Structure):
+    """struct ssc_adamw_tensor."""
+    _fields_ = [("param", _vp), ("grad", _vp), ("exp_avg", _vp), ("exp_avg_sq", _vp),
+                ("exp_avg_scale", _vp), ("exp_avg_sq_scale", _vp), ("numel", _i64),
+                ("dtype", _i64)]
+
+
+_dbl = ctypes.c_double
+
 _SIGNATURES = {
     "ssc_version": (ctypes.c_int, []),
     "ssc_last_error": (ctypes.c_char_p, []),
@@ -178,6 +188,13 @@ _SIGNATURES = {
     "ssc_field_scale_f32": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp]),
     "ssc_bnact_bwd_f32": (ctypes.c_int, [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
                                          _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "ssc_groupnorm_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "ssc_groupnorm_fwd": (ctypes.c_int, [_i32, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _vp, _vp,
+                                         ctypes.c_float, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ssc_groupnorm_bwd": (ctypes.c_int, [_i32, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _vp,
+                                         _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ssc_adamw_step": (ctypes.c_int, [_vp, _i32, _i32, _dbl, _dbl, _dbl, _dbl, _dbl, _i64, _vp]),
+    "ssc_adamw_values": (ctypes.c_int, [_vp, _i32, _vp]),
 }
 
 for _name, (_res, _args) in _SIGNATURES.items():
@@ -1847,6 +1864,63 @@ def field_scale(x, scale, field_of):
     _check(_lib.ssc_field_scale_f32(_ptr(x), n, c, _ptr(scale), scale.size(1), _ptr(field_of),
                                     _ptr(y), _stream(x)))
     return y
+
+
+# Element types and activations of the pointwise operators (SSC_F32 .., SSC_ACT_SILU ..).
+ELEM = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+ACT_SILU, ACT_GELU = 4, 5
+
+
+def on_device_of(t):
+    """A context in which native launches go to the device of `t`."""
+    return torch.cuda.device(t.device)
+
+
+def groupnorm_forward(x, offsets, groups, weight, bias, eps, act):
+    """y[n, c], mean[clouds, groups], rstd[clouds, groups] of contiguous rows x[n, c]."""
+    n, c = x.shape
+    clouds = offsets.numel() - 1
+    y = torch.empty_like(x)
+    stats = torch.empty((2, clouds, groups), dtype=torch.float32, device=x.device)
+    mean, rstd = stats.unbind()
+    ws = _workspace(_lib.ssc_groupnorm_workspace_bytes(n, c, clouds, groups), x.device)
+    wtype = ELEM[(x if weight is None else weight).dtype] if bias is None else ELEM[bias.dtype]
+    _check(_lib.ssc_groupnorm_fwd(
+        ELEM[x.dtype], _ptr(x), n, c, offsets.data_ptr(), clouds, groups, wtype, _ptr(weight),
+        _ptr(bias), eps, act, _ptr(y), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), ws.numel(),
+        _stream(x)))
+    return y, mean, rstd
+
+
+def groupnorm_backward(x, dy, offsets, groups, weight, bias, act, mean, rstd, want):
+    """dx, dweight, dbias (None where `want` says so) of contiguous rows x, dy [n, c], n >= 1."""
+    n, c = x.shape
+    clouds = offsets.numel() - 1
+    dx = torch.empty_like(x) if want[0] else None
+    dweight = torch.empty_like(weight) if want[1] else None
+    dbias = torch.empty_like(bias) if want[2] else None
+    ws = _workspace(_lib.ssc_groupnorm_workspace_bytes(n, c, clouds, groups), x.device)
+    wtype = ELEM[(x if weight is None else weight).dtype] if bias is None else ELEM[bias.dtype]
+    _check(_lib.ssc_groupnorm_bwd(
+        ELEM[x.dtype], x.data_ptr(), dy.data_ptr(), n, c, offsets.data_ptr(), clouds, groups, wtype,
+        _ptr(weight), _ptr(bias), act, mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dweight),
+        _ptr(dbias), ws.data_ptr(), ws.numel(), _stream(x)))
+    return dx, dweight, dbias
+
+
+def adamw_table(rows):
+    """An array of ssc_adamw_tensor from (param, grad, exp_avg, exp_avg_sq, scale, scale, numel,
+    element type) of every tensor, addresses as integers."""
+    return (AdamwTensor * len(rows))(*rows)
+
+
+def adamw_step(table, state_bits, lr, beta1, beta2, eps, weight_decay, step, stream):
+    _check(_lib.ssc_adamw_step(table, len(table), state_bits, lr, beta1, beta2, eps, weight_decay,
+                               step, stream))
+
+
+def adamw_values(table, stream):
+    _check(_lib.ssc_adamw_values(table, len(table), stream))
 
 
 def profile_conv(enable, every=1):
