@@ -1,0 +1,642 @@
+// Gated feed-forward block: y = act(x w_gate^T + b_gate) * (x w_up^T + b_up), and its gradients.
+//
+// With a = x w_gate^T + b_gate, b = x w_up^T + b_up:
+//   db = dy act(a), da = dy b act'(a)
+//   dx = da w_gate + db w_up, dw_gate = da^T x, dw_up = db^T x, db_gate, db_up = column sums.
+//
+// Forward: one launch of the matrix kernel (gated_gemm.h) whose tiles hold the same columns of
+// both projections, so activation and product happen in registers and neither projection goes
+// through memory (a training step keeps a and b, in the rows' type, for the backward pass); up to
+// kFewRows rows a kernel that streams the weights once.  Backward: one pass makes da and db, side
+// by side along k and once more transposed, then one product gives dx (k runs over both
+// projections' columns) and one gives both weight gradients (k runs over the rows, cut into
+// slices where there are few tiles; slices are added in order).
+// 16-bit elements: matrix-bound for many rows, bound by the weights' bytes for few.
+#include "gated_gemm.h"
+
+namespace ssc {
+namespace {
+
+constexpr int kFewRows = 32;
+
+// ---- operands of the matrix kernel ----------------------------------------------------------
+// How an element of the user's arrays becomes PARTS 16-bit ones.
+template <typename T> struct Split {
+  typedef T P;
+  static constexpr int PARTS = 1;
+  static __device__ __forceinline__ void of(float v, P *p) { p[0] = (T)v; }
+};
+template <> struct Split<float> {
+  typedef bf16 P;
+  static constexpr int PARTS = 3;
+  static __device__ __forceinline__ void of(float v, P *p) {
+    p[0] = (bf16)v;
+    // the largest floats would round to infinity: cut instead
+    if (__builtin_isfinite(v) && !__builtin_isfinite((float)p[0]))
+      p[0] = (bf16)__uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
+    const float r = v - (float)p[0];
+    const bool fine = __builtin_isfinite(r);  // (of an infinity or NaN nothing is left)
+    p[1] = fine ? (bf16)r : (bf16)0.f;
+    p[2] = fine ? (bf16)(r - (float)p[1]) : (bf16)0.f;
+  }
+};
+
+// 8 values as a chunk of each part; parts lie `stride` elements apart.
+template <typename T>
+__device__ __forceinline__ void put_chunk(typename Split<T>::P *to, int64_t stride, const float *v) {
+  typedef typename Split<T>::P P;
+  P parts[8][Split<T>::PARTS];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) Split<T>::of(v[i], parts[i]);
+#pragma unroll
+  for (int p = 0; p < Split<T>::PARTS; ++p) {
+    typename Pack<P, 8>::type c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = parts[i][p];
+    *reinterpret_cast<typename Pack<P, 8>::type *>(to + p * stride) = c;
+  }
+}
+
+// src [rows, cols] -> dst [rows][PARTS][padded]: for rows that are no multiple of 16 bytes, and
+// for floats.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    pack_rows_kernel(const T *__restrict__ src, int64_t rows, int64_t cols, int64_t padded,
+                     typename Split<T>::P *__restrict__ dst) {
+  const int64_t chunks = padded / 8, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= rows * chunks) return;
+  const int64_t r = at / chunks, c = (at - r * chunks) * 8;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? (float)src[r * cols + c + i] : 0.f;
+  put_chunk<T>(dst + (r * Split<T>::PARTS) * padded + c, padded, v);
+}
+
+constexpr int kT = 64;  // edge of the tiles that are transposed
+// Writes a tile t[row][col] (kT x kT, in LDS) transposed: columns c0 .. of dst [cols][PARTS][ld],
+// rows r0 ... as its k; `padded` bounds k (a multiple of 8), `cols` the columns.
+template <typename T>
+__device__ __forceinline__ void put_transposed(const float (*t)[kT + 1], int64_t r0, int64_t padded,
+                                               int64_t c0, int64_t cols, int64_t ld,
+                                               typename Split<T>::P *__restrict__ dst) {
+  for (int i = threadIdx.x; i < kT * (kT / 8); i += 256) {
+    const int c = i / (kT / 8), r = i % (kT / 8) * 8;
+    if (c0 + c >= cols || r0 + r >= padded) continue;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = t[r + e][c];
+    put_chunk<T>(dst + (c0 + c) * Split<T>::PARTS * ld + r0 + r, ld, v);
+  }
+}
+
+// src [rows, cols] -> dst [cols][PARTS][ld], k = rows at `offset`; blockIdx.z: two sources whose
+// rows lie side by side (offset, 2 offset).
+template <typename T>
+__global__ void __launch_bounds__(256)
+    pack_transposed_kernel(const T *__restrict__ src0, const T *__restrict__ src1, int64_t rows,
+                           int64_t cols, int64_t padded, int64_t ld,
+                           typename Split<T>::P *__restrict__ dst) {
+  __shared__ float t[kT][kT + 1];
+  const T *src = blockIdx.z == 0 ? src0 : src1;
+  dst += blockIdx.z * padded;
+  const int64_t r0 = (int64_t)blockIdx.x * kT, c0 = (int64_t)blockIdx.y * kT;
+  const int c = threadIdx.x & 63;
+  for (int r = threadIdx.x >> 6; r < kT; r += 4)
+    t[r][c] = r0 + r < rows && c0 + c < cols ? (float)src[(r0 + r) * cols + c0 + c] : 0.f;
+  __syncthreads();
+  put_transposed<T>(t, r0, padded, c0, cols, ld, dst);
+}
+
+// da and db of a tile of 64 rows x 64 hidden columns.
+//   g  [m][PARTS][2 hp]: da at k = 0 .., db at k = hp ..  (NULL: not wanted)
+//   gt [2 h][PARTS][mp]: rows 0 .. of da, h .. of db      (NULL: not wanted)
+//   sums [tiles of rows][2 h]: column sums of the tile    (NULL: not wanted)
+template <typename T>
+__global__ void __launch_bounds__(256)
+    gated_grad_kernel(const T *__restrict__ dy, const T *__restrict__ a, const T *__restrict__ b,
+                      int64_t m, int64_t h, int act, int64_t hp, int64_t mp,
+                      typename Split<T>::P *__restrict__ g, typename Split<T>::P *__restrict__ gt,
+                      float *__restrict__ sums) {
+  __shared__ float ta[kT][kT + 1], tb[kT][kT + 1];
+  const int64_t r0 = (int64_t)blockIdx.x * kT, c0 = (int64_t)blockIdx.y * kT;
+  const int c = threadIdx.x & 63;
+  for (int r = threadIdx.x >> 6; r < kT; r += 4) {
+    float da = 0.f, db = 0.f;
+    if (r0 + r < m && c0 + c < h) {
+      const int64_t at = (r0 + r) * h + c0 + c;
+      const float y = (float)dy[at], av = (float)a[at], bv = (float)b[at];
+      float f, d;
+      activate_slope<1>(act, &av, &f, &d);
+      db = y * f;
+      da = y * bv * d;
+    }
+    ta[r][c] = da;
+    tb[r][c] = db;
+  }
+  __syncthreads();
+  if (sums != nullptr && threadIdx.x < 128) {
+    const float (*t)[kT + 1] = threadIdx.x < 64 ? ta : tb;
+    float s = 0.f;
+    for (int r = 0; r < kT; ++r) s += t[r][c];
+    if (c0 + c < h) sums[(int64_t)blockIdx.x * 2 * h + (threadIdx.x < 64 ? 0 : h) + c0 + c] = s;
+  }
+  if (g != nullptr)
+    for (int i = threadIdx.x; i < 2 * kT * (kT / 8); i += 256) {
+      const int which = i / (kT * (kT / 8)), r = i / (kT / 8) % kT, k = i % (kT / 8) * 8;
+      if (r0 + r >= m || c0 + k >= hp) continue;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = which == 0 ? ta[r][k + e] : tb[r][k + e];
+      put_chunk<T>(g + (r0 + r) * Split<T>::PARTS * 2 * hp + which * hp + c0 + k, 2 * hp, v);
+    }
+  if (gt != nullptr) {
+    put_transposed<T>(ta, r0, mp, c0, h, mp, gt);
+    put_transposed<T>(tb, r0, mp, c0, h, mp, gt + h * Split<T>::PARTS * mp);
+  }
+}
+
+// Column sums of the row tiles, added in order: 64 columns of a workgroup, 4 runs of tiles.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    bias_grad_kernel(const float *__restrict__ sums, int64_t tiles, int64_t h, T *__restrict__ db_gate,
+                     T *__restrict__ db_up) {
+  __shared__ float t[4][64];
+  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int run = threadIdx.x >> 6;
+  float s = 0.f;
+  if (c < 2 * h)
+    for (int64_t r = run; r < tiles; r += 4) s += sums[r * 2 * h + c];
+  t[run][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (run == 0 && c < 2 * h) {
+    const int x = threadIdx.x;
+    s = (t[0][x] + t[1][x]) + (t[2][x] + t[3][x]);
+    if (c < h) {
+      if (db_gate) db_gate[c] = (T)s;
+    } else if (db_up) {
+      db_up[c - h] = (T)s;
+    }
+  }
+}
+
+// Slices of a product added in order, rounded once.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    add_slices_kernel(const float *__restrict__ part, int slices, int64_t count, int64_t split,
+                      T *__restrict__ out, T *__restrict__ out2) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  float s = 0.f;
+  for (int z = 0; z < slices; ++z) s += part[z * count + i];
+  if (i < split) out[i] = (T)s;
+  else out2[i - split] = (T)s;
+}
+
+// ---- few rows -------------------------------------------------------------------------------
+// 16 hidden columns of both projections, up to 16 MT rows; the waves of the workgroup take the
+// steps along k in turn and are added up in LDS.  Bound by the weights' bytes: a lane reads 32
+// neighbouring bytes of a row of the weights at a step, and rows (16 lanes) and steps are
+// independent, so many loads are in flight.  k is dealt to the lanes as the weights lie in
+// memory, not in the matrix instruction's own order: a sum does not mind as long as x is dealt
+// alike.
+template <typename T> struct FewStep;  // one step: 64 elements along k (16 bits), 32 (float)
+template <> struct FewStep<f16> { static constexpr int kLane = 16; };
+template <> struct FewStep<bf16> { static constexpr int kLane = 16; };
+template <> struct FewStep<float> { static constexpr int kLane = 8; };
+
+// kLane elements from p, of which `left` exist (the rest count as zero).
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void few_load(const T *p, int64_t left, T *v) {
+  constexpr int L = FewStep<T>::kLane, V = 16 / sizeof(T);
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int i = 0; i < L; i += V) {
+      typename Pack<T, V>::type c = {};
+      if (i < left) c = *reinterpret_cast<const typename Pack<T, V>::type *>(p + i);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i + e] = c[e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < L; ++i) v[i] = i < left ? p[i] : (T)0.f;
+  }
+}
+
+__device__ __forceinline__ void few_mul(const float *w, const float *x, f32x4 &acc) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i], x[i], acc, 0, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ void few_mul(const T *w, const T *x, f32x4 &acc) {
+  typedef typename Frag<T>::type F;
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    F wf, xf;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      wf[e] = w[i + e];
+      xf[e] = x[i + e];
+    }
+    acc = mfma16(wf, xf, acc);
+  }
+}
+
+template <typename T, int MT, bool ALIGNED>
+__global__ void __launch_bounds__(512) few_rows_kernel(const GemmArgs g) {
+  constexpr int L = FewStep<T>::kLane, W = 8;
+  __shared__ f32x4 lds[W][2 * MT][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t col = n0 + r < g.n ? n0 + r : g.n - 1;
+  const T *wg = static_cast<const T *>(g.b) + col * g.ldb, *wu = static_cast<const T *>(g.b2) + col * g.ldb;
+  const T *x[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+    x[t] = static_cast<const T *>(g.a) + (t * 16 + r < g.m ? t * 16 + r : g.m - 1) * g.lda;
+  f32x4 acc[2 * MT];
+#pragma unroll
+  for (int t = 0; t < 2 * MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int k0 = w * 4 * L;
+#pragma unroll 2
+  for (; k0 + 4 * L <= g.k; k0 += W * 4 * L) {
+    T gv[L], uv[L], xv[MT][L];
+    const int k = k0 + q * L;
+    few_load<T, ALIGNED>(wg + k, L, gv);
+    few_load<T, ALIGNED>(wu + k, L, uv);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) few_load<T, ALIGNED>(x[t] + k, L, xv[t]);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      few_mul(gv, xv[t], acc[2 * t]);
+      few_mul(uv, xv[t], acc[2 * t + 1]);
+    }
+  }
+  if (k0 < g.k) {
+    T gv[L], uv[L], xv[MT][L];
+    const int k = k0 + q * L;
+    few_load<T, ALIGNED>(wg + k, g.k - k, gv);
+    few_load<T, ALIGNED>(wu + k, g.k - k, uv);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      few_load<T, ALIGNED>(x[t] + k, g.k - k, xv[t]);
+      few_mul(gv, xv[t], acc[2 * t]);
+      few_mul(uv, xv[t], acc[2 * t + 1]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 2 * MT; ++t) lds[w][t][lane] = acc[t];
+  __syncthreads();
+  if (w >= MT) return;
+  f32x4 sa = lds[0][2 * w][lane], sb = lds[0][2 * w + 1][lane];
+#pragma unroll
+  for (int v = 1; v < W; ++v) {
+    sa += lds[v][2 * w][lane];
+    sb += lds[v][2 * w + 1][lane];
+  }
+  const int64_t row = w * 16 + r, c0 = n0 + q * 4;
+  if (row >= g.m) return;
+  float a[4], b[4], f[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool in = c0 + e < g.n;
+    a[e] = sa[e] + (g.bias_a && in ? (float)static_cast<const T *>(g.bias_a)[c0 + e] : 0.f);
+    b[e] = sb[e] + (g.bias_b && in ? (float)static_cast<const T *>(g.bias_b)[c0 + e] : 0.f);
+  }
+  activate<4>(g.act, a, f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c0 + e < g.n) {
+      const int64_t at = row * g.ldo + c0 + e;
+      static_cast<T *>(g.out)[at] = (T)(f[e] * b[e]);
+      if (g.pre_a) {
+        static_cast<T *>(g.pre_a)[at] = (T)a[e];
+        static_cast<T *>(g.pre_b)[at] = (T)b[e];
+      }
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------
+int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
+bool at16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Tiles: large ones reuse more of what they read, small ones fill the chip where there are few.
+template <typename T> struct Tiles {
+  typedef Tile<T, 1, 256, 256, 64, 2, 4> Large;
+  typedef Tile<T, 1, 128, 128, 64, 2, 2> Middle;
+  typedef Tile<T, 1, 64, 128, 64, 1, 4> Small;
+};
+template <> struct Tiles<float> {
+  typedef Tile<bf16, 3, 256, 128, 32, 4, 2> Large;
+  typedef Tile<bf16, 3, 128, 128, 32, 2, 2> Middle;
+  typedef Tile<bf16, 3, 64, 128, 32, 1, 4> Small;
+};
+constexpr int kCUs = 256;
+
+template <typename C> int64_t tiles_of(int64_t m, int64_t n) {
+  return ceil_div(m, C::BM) * ceil_div(n, C::BN);
+}
+
+struct Shape {
+  int64_t m, n, k;
+};
+
+// Slices along k of a product with too few tiles to fill the chip (at least 4 steps each).
+template <typename C> int slices_of(const Shape &s) {
+  const int64_t tiles = tiles_of<C>(s.m, s.n), steps = ceil_div(s.k, C::BK);
+  int64_t z = tiles >= kCUs ? 1 : 2 * kCUs / tiles;
+  if (z > steps / 4) z = steps / 4;
+  if (z < 1) z = 1;
+  return (int)ceil_div(steps, ceil_div(steps, z));
+}
+// 2: large tiles, 1: middle ones, 0: small ones
+template <typename T> int size_of(const Shape &s, bool sliced) {
+  if (sliced) {
+    // (work per tile counts: a sliced product fills the chip with any of them)
+    if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) * s.k >= (int64_t)kCUs * 2048) return 2;
+    return s.m > 64 ? 1 : 0;
+  }
+  if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) >= kCUs) return 2;
+  if (tiles_of<typename Tiles<T>::Middle>(s.m, s.n) >= kCUs) return 1;
+  return 0;
+}
+template <typename T> int slices_for(const Shape &s) {
+  const int z = size_of<T>(s, true);
+  return z == 2 ? slices_of<typename Tiles<T>::Large>(s)
+                : z == 1 ? slices_of<typename Tiles<T>::Middle>(s) : slices_of<typename Tiles<T>::Small>(s);
+}
+
+template <typename C, int EPI, typename O>
+int launch(GemmArgs g, int64_t n_tile, int slices, hipStream_t s) {
+  g.tiles_m = (int32_t)ceil_div(g.m, C::BM);
+  g.tiles_n = (int32_t)ceil_div(n_tile, C::BN);
+  SSC_CHECK((int64_t)g.tiles_m * g.tiles_n <= 0x7FFFFFFF, SSC_EINVAL, "too many tiles");
+  g.kslice = (int32_t)(ceil_div(ceil_div(g.k, C::BK), slices) * C::BK);
+  hipLaunchKernelGGL((gemm_kernel<C, EPI, O>), dim3(g.tiles_m * g.tiles_n, 1, slices), dim3(C::kThreads),
+                     0, s, g);
+  SSC_LAUNCH_CHECK("gated feed-forward product");
+  return SSC_OK;
+}
+
+// A product whose result goes to out / out2 (rows from split on), in slices where that pays.
+template <typename T>
+int product(GemmArgs g, float *part, hipStream_t s) {
+  const Shape shape = {g.m, g.n, g.k};
+  const int size = size_of<T>(shape, true), slices = slices_for<T>(shape);
+  typedef Tiles<T> S;
+  if (slices == 1) {
+    g.wide = (g.ldo * sizeof(T)) % 16 == 0 && at16(g.out) && (g.out2 == nullptr || at16(g.out2));
+    return size == 2 ? launch<typename S::Large, kStore, T>(g, g.n, 1, s)
+                     : size == 1 ? launch<typename S::Middle, kStore, T>(g, g.n, 1, s)
+                                 : launch<typename S::Small, kStore, T>(g, g.n, 1, s);
+  }
+  GemmArgs p = g;
+  p.out = part;
+  p.wide = g.ldo % 4 == 0;
+  const int rc = size == 2 ? launch<typename S::Large, kPartial, float>(p, g.n, slices, s)
+                           : size == 1 ? launch<typename S::Middle, kPartial, float>(p, g.n, slices, s)
+                                       : launch<typename S::Small, kPartial, float>(p, g.n, slices, s);
+  if (rc != SSC_OK) return rc;
+  const int64_t count = g.m * g.n;
+  hipLaunchKernelGGL(add_slices_kernel<T>, dim3((uint32_t)ceil_div(count, 256)), dim3(256), 0, s, part,
+                     slices, count, g.out2 ? g.split * g.n : count, static_cast<T *>(g.out),
+                     static_cast<T *>(g.out2));
+  SSC_LAUNCH_CHECK("add_slices_kernel");
+  return SSC_OK;
+}
+
+template <typename T>
+int pack_rows(const void *src, int64_t rows, int64_t cols, int64_t padded, void *dst, hipStream_t s) {
+  hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((uint32_t)ceil_div(rows * (padded / 8), 256)), dim3(256), 0,
+                     s, static_cast<const T *>(src), rows, cols, padded,
+                     static_cast<typename Split<T>::P *>(dst));
+  SSC_LAUNCH_CHECK("pack_rows_kernel");
+  return SSC_OK;
+}
+
+// Whether the matrix kernel reads the user's rows as they are.
+template <typename T> bool reads_plain(int64_t k, const void *x, const void *wg, const void *wu) {
+  return Split<T>::PARTS == 1 && k % 8 == 0 && at16(x) && at16(wg) && at16(wu);
+}
+
+struct Problem {
+  int64_t m, k, h;
+};
+
+size_t packed_bytes(int64_t rows, int64_t padded, int parts) {
+  return align_up((size_t)rows * padded * parts * 2);
+}
+
+template <typename T> size_t forward_bytes(const Problem &p) {
+  if (p.m <= kFewRows) return 256;
+  const int64_t kp = up8(p.k);
+  return packed_bytes(p.m, kp, Split<T>::PARTS) + 2 * packed_bytes(p.h, kp, Split<T>::PARTS);
+}
+
+template <typename T, bool ALIGNED> void few_rows(const GemmArgs &g, hipStream_t s) {
+  const dim3 grid((uint32_t)ceil_div(g.n, 16));
+  if (g.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, ALIGNED>), grid, dim3(512), 0, s, g);
+  else hipLaunchKernelGGL((few_rows_kernel<T, 2, ALIGNED>), grid, dim3(512), 0, s, g);
+}
+
+template <typename T>
+int forward(const Problem &p, const void *x, const void *wg, const void *wu, const void *bg,
+            const void *bu, int act, void *y, void *a, void *b, void *ws, hipStream_t s) {
+  GemmArgs g = {};
+  g.m = p.m;
+  g.n = p.h;
+  g.bias_a = bg;
+  g.bias_b = bu;
+  g.act = act;
+  g.out = y;
+  g.pre_a = a;
+  g.pre_b = b;
+  g.ldo = p.h;
+  if (p.m <= kFewRows) {
+    g.a = x;
+    g.b = wg;
+    g.b2 = wu;
+    g.k = (int32_t)p.k;
+    g.lda = g.ldb = p.k;
+    const bool aligned = (p.k * sizeof(T)) % 16 == 0 && at16(x) && at16(wg) && at16(wu);
+    if (aligned) few_rows<T, true>(g, s);
+    else few_rows<T, false>(g, s);
+    SSC_LAUNCH_CHECK("few_rows_kernel");
+    return SSC_OK;
+  }
+  const int64_t kp = up8(p.k);
+  g.k = (int32_t)kp;
+  g.lda = g.ldb = kp * Split<T>::PARTS;
+  if (reads_plain<T>(p.k, x, wg, wu)) {
+    g.a = x;
+    g.b = wg;
+    g.b2 = wu;
+  } else {
+    typedef typename Split<T>::P P;
+    Carver c(ws);
+    P *xp = c.take<P>(p.m * g.lda), *gp = c.take<P>(p.h * g.lda), *up = c.take<P>(p.h * g.lda);
+    int rc = pack_rows<T>(x, p.m, p.k, kp, xp, s);
+    if (rc == SSC_OK) rc = pack_rows<T>(wg, p.h, p.k, kp, gp, s);
+    if (rc == SSC_OK) rc = pack_rows<T>(wu, p.h, p.k, kp, up, s);
+    if (rc != SSC_OK) return rc;
+    g.a = xp;
+    g.b = gp;
+    g.b2 = up;
+  }
+  g.wide = (p.h * sizeof(T)) % 16 == 0 && at16(y) && at16(a) && at16(b);
+  const int size = size_of<T>({p.m, 2 * p.h, kp}, false);
+  typedef Tiles<T> S;
+  return size == 2 ? launch<typename S::Large, kGated, T>(g, 2 * p.h, 1, s)
+                   : size == 1 ? launch<typename S::Middle, kGated, T>(g, 2 * p.h, 1, s)
+                               : launch<typename S::Small, kGated, T>(g, 2 * p.h, 1, s);
+}
+
+template <typename T> struct Backward {
+  typedef typename Split<T>::P P;
+  static constexpr int PARTS = Split<T>::PARTS;
+  int64_t hp, mp;
+  P *g, *gt, *wt, *xt;
+  float *sums, *part;
+  size_t bytes;
+  Backward(const Problem &p, void *ws) {
+    hp = up8(p.h);
+    mp = up8(p.m);
+    Carver c(ws);
+    g = c.take<P>(p.m * PARTS * 2 * hp);
+    gt = c.take<P>(2 * p.h * PARTS * mp);
+    wt = c.take<P>(p.k * PARTS * 2 * hp);
+    xt = c.take<P>(p.k * PARTS * mp);
+    sums = c.take<float>(ceil_div(p.m, kT) * 2 * p.h);
+    // the slices of the two products, one after the other
+    const Shape sx = {p.m, p.k, 2 * hp}, sw = {2 * p.h, p.k, mp};
+    const int zx = slices_for<T>(sx), zw = slices_for<T>(sw);
+    const int64_t px = zx > 1 ? zx * p.m * p.k : 0, pw = zw > 1 ? zw * 2 * p.h * p.k : 0;
+    part = c.take<float>(px > pw ? px : pw);
+    bytes = c.used;
+  }
+};
+
+template <typename T>
+int backward(const Problem &p, const void *x, const void *wg, const void *wu, int act, const void *a,
+             const void *b, const void *dy, void *dx, void *dwg, void *dwu, void *dbg, void *dbu,
+             void *ws, hipStream_t s) {
+  typedef typename Split<T>::P P;
+  constexpr int PARTS = Split<T>::PARTS;
+  const Backward<T> w(p, ws);
+  const bool weights = dwg != nullptr, biases = dbg != nullptr || dbu != nullptr;
+  const dim3 tiles((uint32_t)ceil_div(p.m, kT), (uint32_t)ceil_div(p.h, kT));
+  hipLaunchKernelGGL(gated_grad_kernel<T>, tiles, dim3(256), 0, s, static_cast<const T *>(dy),
+                     static_cast<const T *>(a), static_cast<const T *>(b), p.m, p.h, act, w.hp, w.mp,
+                     dx ? w.g : nullptr, weights ? w.gt : nullptr, biases ? w.sums : nullptr);
+  SSC_LAUNCH_CHECK("gated_grad_kernel");
+  if (biases) {
+    hipLaunchKernelGGL(bias_grad_kernel<T>, dim3((uint32_t)ceil_div(2 * p.h, 64)), dim3(256), 0, s, w.sums,
+                       ceil_div(p.m, kT), p.h, static_cast<T *>(dbg), static_cast<T *>(dbu));
+    SSC_LAUNCH_CHECK("bias_grad_kernel");
+  }
+  GemmArgs g = {};
+  if (dx) {
+    hipLaunchKernelGGL(pack_transposed_kernel<T>,
+                       dim3((uint32_t)ceil_div(p.h, kT), (uint32_t)ceil_div(p.k, kT), 2), dim3(256), 0, s,
+                       static_cast<const T *>(wg), static_cast<const T *>(wu), p.h, p.k, w.hp, 2 * w.hp,
+                       w.wt);
+    SSC_LAUNCH_CHECK("pack_transposed_kernel");
+    g.a = w.g;
+    g.b = w.wt;
+    g.m = p.m;
+    g.n = p.k;
+    g.k = (int32_t)(2 * w.hp);
+    g.lda = g.ldb = PARTS * 2 * w.hp;
+    g.out = dx;
+    g.split = p.m;
+    g.ldo = p.k;
+    const int rc = product<T>(g, w.part, s);
+    if (rc != SSC_OK) return rc;
+  }
+  if (weights) {
+    hipLaunchKernelGGL(pack_transposed_kernel<T>,
+                       dim3((uint32_t)ceil_div(p.m, kT), (uint32_t)ceil_div(p.k, kT), 1), dim3(256), 0, s,
+                       static_cast<const T *>(x), static_cast<const T *>(x), p.m, p.k, w.mp, w.mp, w.xt);
+    SSC_LAUNCH_CHECK("pack_transposed_kernel");
+    g.a = w.gt;
+    g.b = w.xt;
+    g.m = 2 * p.h;
+    g.n = p.k;
+    g.k = (int32_t)w.mp;
+    g.lda = g.ldb = PARTS * w.mp;
+    g.out = dwg;
+    g.out2 = dwu;
+    g.split = p.h;
+    g.ldo = p.k;
+    const int rc = product<T>(g, w.part, s);
+    if (rc != SSC_OK) return rc;
+  }
+  return SSC_OK;
+}
+
+// What 32-bit offsets inside a few rows allow.
+constexpr int64_t kMostAlong = 1 << 24;
+
+int check(int32_t dtype, int64_t m, int64_t k, int64_t h, int32_t act) {
+  SSC_CHECK(dtype_ok(dtype), SSC_EINVAL, "element type %d", dtype);
+  SSC_CHECK(m >= 0 && k >= 1 && h >= 1, SSC_EINVAL, "%lld rows, widths %lld and %lld", (long long)m,
+            (long long)k, (long long)h);
+  SSC_CHECK(m <= kMostAlong && k <= kMostAlong / 8 && h <= kMostAlong / 8, SSC_EINVAL,
+            "%lld rows, widths %lld and %lld: at most %lld and %lld", (long long)m, (long long)k,
+            (long long)h, (long long)kMostAlong, (long long)(kMostAlong / 8));
+  SSC_CHECK(pointwise_act_ok(act), SSC_EINVAL, "activation %d", act);
+  return SSC_OK;
+}
+
+}  // namespace
+}  // namespace ssc
+
+using namespace ssc;
+
+extern "C" size_t ssc_gated_fwd_workspace_bytes(int32_t dtype, int64_t m, int64_t k, int64_t h) {
+  const Problem p = {m, k, h};
+  return dtype == SSC_F32 ? forward_bytes<float>(p) : forward_bytes<f16>(p);
+}
+
+extern "C" int ssc_gated_fwd(int32_t dtype, const void *x, int64_t m, int64_t k, const void *w_gate,
+                             const void *w_up, int64_t h, const void *b_gate, const void *b_up,
+                             int32_t act, void *y, void *a, void *b, void *ws, size_t ws_bytes,
+                             ssc_stream_t stream) {
+  const int rc = check(dtype, m, k, h, act);
+  if (rc != SSC_OK) return rc;
+  if (m == 0) return SSC_OK;
+  SSC_CHECK(x && w_gate && w_up && y && (a == nullptr) == (b == nullptr), SSC_EINVAL, "NULL pointer");
+  SSC_CHECK(ws != nullptr && ws_bytes >= ssc_gated_fwd_workspace_bytes(dtype, m, k, h), SSC_EWORKSPACE,
+            "workspace of %zu bytes, %zu are needed", ws_bytes,
+            ssc_gated_fwd_workspace_bytes(dtype, m, k, h));
+  const Problem p = {m, k, h};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == SSC_F32) return forward<float>(p, x, w_gate, w_up, b_gate, b_up, act, y, a, b, ws, s);
+  if (dtype == SSC_F16) return forward<f16>(p, x, w_gate, w_up, b_gate, b_up, act, y, a, b, ws, s);
+  return forward<bf16>(p, x, w_gate, w_up, b_gate, b_up, act, y, a, b, ws, s);
+}
+
+extern "C" size_t ssc_gated_bwd_workspace_bytes(int32_t dtype, int64_t m, int64_t k, int64_t h) {
+  if (m <= 0) return 256;
+  const Problem p = {m, k, h};
+  return dtype == SSC_F32 ? Backward<float>(p, nullptr).bytes : Backward<f16>(p, nullptr).bytes;
+}
+
+extern "C" int ssc_gated_bwd(int32_t dtype, const void *x, int64_t m, int64_t k, const void *w_gate,
+                             const void *w_up, int64_t h, int32_t act, const void *a, const void *b,
+                             const void *dy, void *dx, void *dw_gate, void *dw_up, void *db_gate,
+                             void *db_up, void *ws, size_t ws_bytes, ssc_stream_t stream) {
+  const int rc = check(dtype, m, k, h, act);
+  if (rc != SSC_OK) return rc;
+  if (m == 0) return SSC_OK;
+  SSC_CHECK(x && w_gate && w_up && a && b && dy && (dw_gate == nullptr) == (dw_up == nullptr), SSC_EINVAL,
+            "NULL pointer");
+  SSC_CHECK(ws != nullptr && ws_bytes >= ssc_gated_bwd_workspace_bytes(dtype, m, k, h), SSC_EWORKSPACE,
+            "workspace of %zu bytes, %zu are needed", ws_bytes,
+            ssc_gated_bwd_workspace_bytes(dtype, m, k, h));
+  const Problem p = {m, k, h};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define SSC_GATED_BWD(T) \
+  backward<T>(p, x, w_gate, w_up, act, a, b, dy, dx, dw_gate, dw_up, db_gate, db_up, ws, s)
+  return dtype == SSC_F32 ? SSC_GATED_BWD(float) : dtype == SSC_F16 ? SSC_GATED_BWD(f16) : SSC_GATED_BWD(bf16);
+#undef SSC_GATED_BWD
+}

@@ -9,7 +9,8 @@ from . import batchnorm
 from . import pool
 from . import dropout
 from . import groupnorm
+from . import feedforward
 from . import optim
 
 __all__ = ["sp_ops", "utils", "convolution", "activation", "batchnorm", "pool", "dropout",
-           "groupnorm", "optim"]
+           "groupnorm", "feedforward", "optim"]

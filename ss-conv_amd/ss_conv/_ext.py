@@ -193,6 +193,12 @@ _SIGNATURES = {
                                          ctypes.c_float, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ssc_groupnorm_bwd": (ctypes.c_int, [_i32, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _vp,
                                          _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ssc_gated_fwd_workspace_bytes": (_sz, [_i32, _i64, _i64, _i64]),
+    "ssc_gated_fwd": (ctypes.c_int, [_i32, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _vp,
+                                     _vp, _vp, _sz, _vp]),
+    "ssc_gated_bwd_workspace_bytes": (_sz, [_i32, _i64, _i64, _i64]),
+    "ssc_gated_bwd": (ctypes.c_int, [_i32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp,
+                                     _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ssc_adamw_step": (ctypes.c_int, [_vp, _i32, _i32, _dbl, _dbl, _dbl, _dbl, _dbl, _i64, _vp]),
     "ssc_adamw_values": (ctypes.c_int, [_vp, _i32, _vp]),
 }
@@ -1906,6 +1912,40 @@ def groupnorm_backward(x, dy, offsets, groups, weight, bias, act, mean, rstd, wa
         _ptr(weight), _ptr(bias), act, mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dweight),
         _ptr(dbias), ws.data_ptr(), ws.numel(), _stream(x)))
     return dx, dweight, dbias
+
+
+def gated_forward(x, w_gate, w_up, b_gate, b_up, act, keep):
+    """y[m, h] of contiguous rows x[m, k]; with `keep` also the projections a, b[m, h] that the
+    backward pass reads (else None)."""
+    m, k = x.shape
+    h = w_gate.size(0)
+    y = x.new_empty((m, h))
+    a = x.new_empty((m, h)) if keep else None
+    b = x.new_empty((m, h)) if keep else None
+    elem = ELEM[x.dtype]
+    ws = _workspace(_lib.ssc_gated_fwd_workspace_bytes(elem, m, k, h), x.device)
+    _check(_lib.ssc_gated_fwd(elem, _ptr(x), m, k, w_gate.data_ptr(), w_up.data_ptr(), h,
+                              _ptr(b_gate), _ptr(b_up), act, _ptr(y), _ptr(a), _ptr(b),
+                              ws.data_ptr(), ws.numel(), _stream(x)))
+    return y, a, b
+
+
+def gated_backward(x, w_gate, w_up, act, a, b, dy, want):
+    """dx, dw_gate, dw_up, db_gate, db_up (None where `want` says so), m >= 1."""
+    m, k = x.shape
+    h = w_gate.size(0)
+    made = lambda like, yes: torch.empty_like(like) if yes else None  # noqa: E731
+    dx = made(x, want[0])
+    weights = want[1] or want[2]  # (one product gives both)
+    dw_gate, dw_up = made(w_gate, weights), made(w_up, weights)
+    db_gate, db_up = [x.new_empty(h) if w else None for w in want[3:5]]
+    elem = ELEM[x.dtype]
+    ws = _workspace(_lib.ssc_gated_bwd_workspace_bytes(elem, m, k, h), x.device)
+    _check(_lib.ssc_gated_bwd(elem, x.data_ptr(), m, k, w_gate.data_ptr(), w_up.data_ptr(), h, act,
+                              a.data_ptr(), b.data_ptr(), dy.data_ptr(), _ptr(dx), _ptr(dw_gate),
+                              _ptr(dw_up), _ptr(db_gate), _ptr(db_up), ws.data_ptr(), ws.numel(),
+                              _stream(x)))
+    return dx, dw_gate if want[1] else None, dw_up if want[2] else None, db_gate, db_up
 
 
 def adamw_table(rows):

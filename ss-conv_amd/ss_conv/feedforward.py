@@ -1,0 +1,118 @@
+"""Gated feed-forward blocks on voxel rows.
+
+    y = act(x w_gate^T + b_gate) * (x w_up^T + b_up)
+
+Both projections, the activation and the product are one kernel (`ssc_gated_fwd`), the gradients
+come from hand-written kernels too (`ssc_gated_bwd`): float32, float16 and bfloat16, sums in
+float32, one rounding of the result.  A training step keeps both projections, rounded to the
+rows' type, for the backward pass.
+
+A block mixes the channels of a row: use it on scalar (order 0) fields, where that keeps the
+network equivariant.
+"""
+import math
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from ss_conv import _ext
+from ss_conv import pointwise
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
+        y, a, b = _ext.gated_forward(x, w_gate, w_up, b_gate, b_up, act, True)
+        ctx.save_for_backward(x, w_gate, w_up, a, b)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w_gate, w_up, a, b = ctx.saved_tensors
+        want = ctx.needs_input_grad[:5]
+        if x.size(0) == 0:
+            shapes = (x, w_gate, w_up, w_gate[:, 0], w_gate[:, 0])
+            return tuple(torch.zeros_like(t) if w else None for t, w in zip(shapes, want)) + (None,)
+        with _ext.on_device_of(x):
+            return _ext.gated_backward(x, w_gate, w_up, ctx.act, a, b, dy.contiguous(), want) + \
+                (None,)
+
+
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
+    """activation(x w_gate^T + b_gate) * (x w_up^T + b_up) for x [..., K] and weights [H, K].
+
+    All tensors have one type (float32, float16 or bfloat16); biases [H] or None.
+    activation: a name (None, "relu", "sigmoid", "tanh", "silu", "gelu"), the torch function or the
+    torch.nn module of one.  Differentiable once in everything."""
+    pointwise.check_rows("x", x)
+    if x.dim() < 1:
+        raise ValueError("x has no dimension")
+    if not torch.is_tensor(w_gate) or w_gate.dim() != 2 or w_gate.size(0) < 1 or \
+            w_gate.size(1) < 1:
+        raise ValueError("w_gate is a matrix [hidden, width]")
+    act = pointwise.activation_code(activation)
+    h, k = w_gate.shape
+    if x.size(-1) != k:
+        raise ValueError("x has {} columns, w_gate {}".format(x.size(-1), k))
+    for what, t, shape in (("w_gate", w_gate, (h, k)), ("w_up", w_up, (h, k)),
+                           ("b_gate", b_gate, (h,)), ("b_up", b_up, (h,))):
+        pointwise.check_like(what, t, shape, (x.dtype,), x.device)
+    if w_up is None:
+        raise TypeError("w_up is missing")
+    rows = x.reshape(-1, k).contiguous()
+    w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+    b_gate, b_up = [None if t is None else t.contiguous() for t in (b_gate, b_up)]
+    with _ext.on_device_of(x):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                           for t in (rows, w_gate, w_up, b_gate, b_up)):
+            y = _GatedLinear.apply(rows, w_gate, w_up, b_gate, b_up, act)
+        else:
+            y = _ext.gated_forward(rows, w_gate, w_up, b_gate, b_up, act, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (h,))
+
+
+class GatedLinear(nn.Module):
+    """gated_linear with its parameters: width columns in, hidden columns out."""
+
+    def __init__(self, width, hidden, bias=False, activation="silu"):
+        super().__init__()
+        self.width, self.hidden = width, hidden
+        self.activation = pointwise.activation_name(activation)
+        self.w_gate = nn.Parameter(torch.empty(hidden, width))
+        self.w_up = nn.Parameter(torch.empty(hidden, width))
+        for name in ("b_gate", "b_up"):
+            self.register_parameter(name, nn.Parameter(torch.empty(hidden)) if bias else None)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        bound = 1 / math.sqrt(self.width)
+        for p in self.parameters():
+            nn.init.uniform_(p, -bound, bound)
+
+    def extra_repr(self):
+        return "{} -> {}, bias={}, activation={}".format(self.width, self.hidden,
+                                                         self.b_gate is not None, self.activation)
+
+    def forward(self, x):
+        return gated_linear(x, self.w_gate, self.w_up, self.b_gate, self.b_up, self.activation)
+
+
+class GatedFeedForward(nn.Module):
+    """x + w_down gated(norm(x)) on the features of a SparseTensor: the residual block of a
+    pointwise network.  norm: a module on SparseTensors (groupnorm.GroupNorm, batchnorm.BatchNorm)
+    or None; the projection back is a plain torch.nn.Linear."""
+
+    def __init__(self, width, hidden, norm=None, bias=False, activation="silu"):
+        super().__init__()
+        self.norm = norm
+        self.gated = GatedLinear(width, hidden, bias, activation)
+        self.down = nn.Linear(hidden, width, bias=bias)
+
+    def forward(self, input):  # pylint: disable=W
+        x = input.features
+        rows = input if self.norm is None else self.norm(input)
+        input.features = x + self.down(self.gated(rows.features))
+        return input
