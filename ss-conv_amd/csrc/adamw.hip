@@ -77,13 +77,15 @@ __device__ __forceinline__ int tensor_of(const int32_t (&first)[N], int count) {
   return __builtin_amdgcn_readfirstlane(below - 1);
 }
 
+// (the quotient by a reciprocal that is right to a unit in the last place: the parameter's own
+// rounding hides it)
 __device__ __forceinline__ void update(const Consts &k, float g, float &p, float &m, float &v,
                                        float &root) {
 #pragma clang fp contract(off)
   m = k.b1 * m + k.omb1 * g;
   v = k.b2 * v + k.omb2 * (g * g);
   root = sqrtf(v);
-  p = p * k.decay - (m / (root * k.root + k.eps)) * k.step;
+  p = p * k.decay - (m * __builtin_amdgcn_rcpf(root * k.root + k.eps)) * k.step;
 }
 
 template <typename T, bool WIDE>
@@ -132,14 +134,21 @@ __global__ void __launch_bounds__(kThreads) adamw32_kernel(const Table<Entry32, 
 }
 
 // Non-negative floats order as their bits do, infinity above every number and NaN above
-// infinity, so a maximum of bits keeps them where a maximum of floats would drop a NaN.
+// infinity, so a maximum of bits keeps them where a maximum of floats would drop a NaN.  Within
+// rows of 16 lanes and then from row to row in the vector unit, without the trips to LDS that a
+// shuffle takes; lane 63 ends with the maximum of all.
+template <int CTRL> __device__ __forceinline__ uint32_t max_with(uint32_t x) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false);
+  return x > o ? x : o;
+}
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t o = __shfl_xor(x, d, 64);
-    x = x > o ? x : o;
-  }
-  return x;
+  x = max_with<0xB1>(x);   // quad_perm 1 0 3 2
+  x = max_with<0x4E>(x);   // quad_perm 2 3 0 1
+  x = max_with<0x141>(x);  // row_half_mirror
+  x = max_with<0x140>(x);  // row_mirror
+  x = max_with<0x142>(x);  // row_bcast:15
+  x = max_with<0x143>(x);  // row_bcast:31
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
 __device__ __forceinline__ float scale_of(uint32_t top, float per_step) {
@@ -147,10 +156,16 @@ __device__ __forceinline__ float scale_of(uint32_t top, float per_step) {
   return fmaxf(__uint_as_float(top) * per_step, FLT_MIN);
 }
 
-// floor(sqrt(x / q) + 1/2)
-__device__ __forceinline__ float code_of(float x, float q) {
+// floor(sqrt(x / q) + 1/2), quotient and root rounded once each.  The quick way, with inv = 1 / q
+// and the hardware's root, is off by less than 4 units of 2^-24 relative, 7e-5 of a code at 255:
+// where it does not lie that near a boundary between two codes both give the same one (all but 3
+// in 10000 values).
+__device__ __forceinline__ float code_of(float x, float q, float inv) {
 #pragma clang fp contract(off)
-  return floorf(sqrtf(x / q) + 0.5f);
+  const float t = __builtin_amdgcn_sqrtf(x * inv) + 0.5f;
+  float c = floorf(t);
+  if (fabsf(t - c - 0.5f) > 0.5f - 1.5e-4f) c = floorf(sqrtf(x / q) + 0.5f);
+  return c;
 }
 
 __device__ __forceinline__ float m_value(int c, float q) { return (float)(c * (c < 0 ? -c : c)) * q; }
@@ -204,11 +219,13 @@ __device__ __forceinline__ void step8(const Entry8 &e, const Consts &k, int64_t 
     mtop = wave_max(mtop);
     vtop = wave_max(vtop);
     const float mn = scale_of(mtop, 1.f / (127.f * 127.f)), vn = scale_of(vtop, 1.f / (255.f * 255.f));
+    // (scales are normal numbers below 2^115, so their reciprocals are normal too)
+    const float mi = __builtin_amdgcn_rcpf(mn), vi = __builtin_amdgcn_rcpf(vn);
     int mc[kPer], vc[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const float a = fminf(code_of(fabsf(mv[j]), mn), 127.f);
-      const float c = fminf(code_of(root[j], vn), 255.f);
+      const float a = fminf(code_of(fabsf(mv[j]), mn, mi), 127.f);
+      const float c = fminf(code_of(root[j], vn, vi), 255.f);
       // (a NaN scale: the codes are 0)
       const int ai = mn == mn ? (int)a : 0;
       mc[j] = mv[j] < 0.f ? -ai : ai;

@@ -155,22 +155,24 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Column sums of the row tiles, added in order: 64 columns of a workgroup, 4 runs of tiles.
+// Column sums of the row tiles, added in order: 16 columns of a workgroup, 16 runs of tiles.
 template <typename T>
 __global__ void __launch_bounds__(256)
     bias_grad_kernel(const float *__restrict__ sums, int64_t tiles, int64_t h, T *__restrict__ db_gate,
                      T *__restrict__ db_up) {
-  __shared__ float t[4][64];
-  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int run = threadIdx.x >> 6;
+  __shared__ float t[16][16];
+  const int x = threadIdx.x & 15, run = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + x;
   float s = 0.f;
-  if (c < 2 * h)
-    for (int64_t r = run; r < tiles; r += 4) s += sums[r * 2 * h + c];
-  t[run][threadIdx.x & 63] = s;
+  if (c < 2 * h) {
+#pragma unroll 8
+    for (int64_t r = run; r < tiles; r += 16) s += sums[r * 2 * h + c];
+  }
+  t[run][x] = s;
   __syncthreads();
   if (run == 0 && c < 2 * h) {
-    const int x = threadIdx.x;
-    s = (t[0][x] + t[1][x]) + (t[2][x] + t[3][x]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) s += t[r][x];
     if (c < h) {
       if (db_gate) db_gate[c] = (T)s;
     } else if (db_up) {
@@ -529,7 +531,7 @@ int backward(const Problem &p, const void *x, const void *wg, const void *wu, in
                      dx ? w.g : nullptr, weights ? w.gt : nullptr, biases ? w.sums : nullptr);
   SSC_LAUNCH_CHECK("gated_grad_kernel");
   if (biases) {
-    hipLaunchKernelGGL(bias_grad_kernel<T>, dim3((uint32_t)ceil_div(2 * p.h, 64)), dim3(256), 0, s, w.sums,
+    hipLaunchKernelGGL(bias_grad_kernel<T>, dim3((uint32_t)ceil_div(2 * p.h, 16)), dim3(256), 0, s, w.sums,
                        ceil_div(p.m, kT), p.h, static_cast<T *>(dbg), static_cast<T *>(dbu));
     SSC_LAUNCH_CHECK("bias_grad_kernel");
   }

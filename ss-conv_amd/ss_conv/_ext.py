@@ -5,7 +5,9 @@ torch supplies device memory and the current stream; all work happens in the
 HIP kernels of the library.  There is no CPU fallback: without the built
 library the import fails, and without a GPU every call raises.
 """
+import array
 import ctypes
+import itertools
 import os
 import threading
 
@@ -34,14 +36,6 @@ class Geometry(ctypes.Structure):
 
 
 _gp = ctypes.POINTER(Geometry)
-
-
-class AdamwTensor(ctypes.Structure):
-    """struct ssc_adamw_tensor."""
-    _fields_ = [("param", _vp), ("grad", _vp), ("exp_avg", _vp), ("exp_avg_sq", _vp),
-                ("exp_avg_scale", _vp), ("exp_avg_sq_scale", _vp), ("numel", _i64),
-                ("dtype", _i64)]
-
 
 _dbl = ctypes.c_double
 
@@ -1948,19 +1942,21 @@ def gated_backward(x, w_gate, w_up, act, a, b, dy, want):
     return dx, dw_gate if want[1] else None, dw_up if want[2] else None, db_gate, db_up
 
 
-def adamw_table(rows):
-    """An array of ssc_adamw_tensor from (param, grad, exp_avg, exp_avg_sq, scale, scale, numel,
-    element type) of every tensor, addresses as integers."""
-    return (AdamwTensor * len(rows))(*rows)
+def adamw_table(columns):
+    """An array of ssc_adamw_tensor, whose fields are eight words each, from the columns param,
+    grad, exp_avg, exp_avg_sq, scale, scale, numel, element type; addresses as integers."""
+    return array.array("q", itertools.chain.from_iterable(zip(*columns)))
 
 
-def adamw_step(table, state_bits, lr, beta1, beta2, eps, weight_decay, step, stream):
-    _check(_lib.ssc_adamw_step(table, len(table), state_bits, lr, beta1, beta2, eps, weight_decay,
-                               step, stream))
+def adamw_step(columns, count, state_bits, lr, beta1, beta2, eps, weight_decay, step, stream):
+    table = adamw_table(columns)
+    _check(_lib.ssc_adamw_step(table.buffer_info()[0], count, state_bits, lr, beta1, beta2, eps,
+                               weight_decay, step, stream))
 
 
-def adamw_values(table, stream):
-    _check(_lib.ssc_adamw_values(table, len(table), stream))
+def adamw_values(columns, count, stream):
+    table = adamw_table(columns)
+    _check(_lib.ssc_adamw_values(table.buffer_info()[0], count, stream))
 
 
 def profile_conv(enable, every=1):

@@ -13,6 +13,9 @@ Sparse gradients, gradients of another type than their parameter and tensors who
 fill their memory one after another are refused.  The number of the step is an argument of the
 launch: a step cannot be captured into a graph and replayed.
 """
+import itertools
+import operator
+
 import torch
 
 from ss_conv import _ext
@@ -66,6 +69,35 @@ def _check_moments(i, n, dev, items, dtypes, sizes):
                              "memory".format(i))
 
 
+def _check_order(i, p, items):
+    for t in items:
+        if t.shape != p.shape or (t.stride() != p.stride() and
+                                  not (t.is_contiguous() and p.is_contiguous())):
+            raise ValueError("moments of tensor {} are laid out as {} {}, their parameter as "
+                             "{} {}".format(i, tuple(t.shape), t.stride(), tuple(p.shape),
+                                            p.stride()))
+
+
+_dtype, _shape, _layout = [operator.attrgetter(n) for n in ("dtype", "shape", "layout")]
+
+
+def _usual(params, lists, dtypes):
+    """Whether all tensors are contiguous, on one GPU and as the checks want them: one pass over
+    each list for each property, where the checks tensor by tensor take several times as long."""
+    shapes = list(map(_shape, params))
+    kinds = list(map(_dtype, params))
+    several = [params] + lists
+    return (all(set(map(_layout, x)) == {torch.strided} for x in several) and
+            all(map(torch.Tensor.is_contiguous, itertools.chain(*several))) and
+            len(set(map(torch.Tensor.get_device, itertools.chain(*several)))) == 1 and
+            params[0].is_cuda and set(kinds) <= _ext.ELEM.keys() and
+            list(map(_dtype, lists[0])) == kinds and
+            all(list(map(_shape, x)) == shapes for x in lists[:3]) and
+            all(set(map(_dtype, x)) == {t} for x, t in zip(lists[1:], dtypes)) and
+            all(list(map(torch.Tensor.numel, x)) == [_scales(p.numel()) for p in params]
+                for x in lists[3:]))
+
+
 _BITS8 = (torch.int8, torch.uint8, torch.float32, torch.float32)
 _BITS32 = (torch.float32, torch.float32)
 
@@ -78,10 +110,10 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.99
            weight_decay=1e-2, exp_avg_scales=None, exp_avg_sq_scales=None):
     """One AdamW step over lists of tensors, all on one device, in place.
 
-    exp_avgs, exp_avg_sqs: the moments, float32 and with as many elements as their parameter;
-    or, with exp_avg_scales and exp_avg_sq_scales (float32, one for each 256 elements), int8
-    and uint8 codes.  A moment's elements belong to the parameter's in the order in which they lie
-    in memory.  step: the number of this step, from 1.  Tensors must not share memory."""
+    exp_avgs, exp_avg_sqs: the moments, float32 and of the shape and strides of their parameter;
+    or, with exp_avg_scales and exp_avg_sq_scales (float32, one for each 256 elements in the order
+    in which they lie in memory), int8 and uint8 codes.  step: the number of this step, from 1.
+    Tensors must not share memory."""
     eight = exp_avg_scales is not None
     if eight != (exp_avg_sq_scales is not None):
         raise ValueError("8-bit moments have scales for both, 32-bit ones have none")
@@ -92,37 +124,31 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.99
             count, [len(x) for x in lists]))
     if count == 0:
         return
+    dtypes = _BITS8 if eight else _BITS32
     dev = params[0].device
-    rows, keep = [], []
-    elem = _ext.ELEM
-    for i, p in enumerate(params):
-        g = grads[i]
-        _check_param(i, p, g)
-        if p.device != dev or g.device != dev:
-            raise RuntimeError("parameter {} is on {}, its gradient on {}, the first on {}".format(
-                i, p.device, g.device, dev))
-        n = p.numel()
-        if g.stride() != p.stride():
-            g = _like(g, p)
-            keep.append(g)
-        m, v = exp_avgs[i], exp_avg_sqs[i]
-        if eight:
-            mq, vq = exp_avg_scales[i], exp_avg_sq_scales[i]
-            _check_moments(i, n, dev, (m, v, mq, vq), _BITS8, (n, n, _scales(n), _scales(n)))
-            rows.append((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), mq.data_ptr(),
-                         vq.data_ptr(), n, elem[p.dtype]))
-        else:
-            _check_moments(i, n, dev, (m, v), _BITS32, (n, n))
-            rows.append((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), None, None, n,
-                         elem[p.dtype]))
+    if not _usual(params, lists, dtypes):
+        lists[0] = grads = list(grads)
+        for i, p in enumerate(params):
+            _check_param(i, p, grads[i])
+            if p.device != dev or grads[i].device != dev:
+                raise RuntimeError("parameter {} is on {}, its gradient on {}, the first on "
+                                   "{}".format(i, p.device, grads[i].device, dev))
+            n = p.numel()
+            _check_moments(i, n, dev, [x[i] for x in lists[1:]], dtypes,
+                           (n, n, _scales(n), _scales(n)))
+            _check_order(i, p, [x[i] for x in lists[1:3]])
+            grads[i] = _like(grads[i], p)
+    columns = [map(torch.Tensor.data_ptr, x) for x in [params] + lists]
+    if not eight:
+        columns += [itertools.repeat(0)] * 2
+    columns += [map(torch.Tensor.numel, params), [_ext.ELEM[p.dtype] for p in params]]
     with torch.cuda.device(dev):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("an AdamW step cannot be captured into a graph: the number of the "
                                "step is an argument of its launch")
-        _ext.adamw_step(_ext.adamw_table(rows), 8 if eight else 32, lr, betas[0], betas[1], eps,
+        _ext.adamw_step(columns, count, 8 if eight else 32, lr, betas[0], betas[1], eps,
                         weight_decay, step, torch.cuda.current_stream(dev).cuda_stream)
-    for p in params:
-        torch.autograd.graph.increment_version(p)
+    torch.autograd.graph.increment_version(params)
 
 
 def state_values(exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, out=None):
@@ -140,20 +166,19 @@ def state_values(exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, out=N
     if out is None:
         out = tuple([torch.empty(t.shape, dtype=torch.float32, device=dev) for t in x]
                     for x in (exp_avgs, exp_avg_sqs))
-    rows = []
+    moments = [exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales]
     for i, m in enumerate(exp_avgs):
         n = m.numel()
-        v, mq, vq = exp_avg_sqs[i], exp_avg_scales[i], exp_avg_sq_scales[i]
-        _check_moments(i, n, dev, (m, v, mq, vq), _BITS8, (n, n, _scales(n), _scales(n)))
+        _check_moments(i, n, dev, [x[i] for x in moments], _BITS8, (n, n, _scales(n), _scales(n)))
         for t in (out[0][i], out[1][i]):
             if t.dtype is not torch.float32 or t.numel() != n or t.device != dev or \
                     not t.is_contiguous():
                 raise ValueError("out of tensor {}: {} contiguous float32 elements are "
                                  "needed".format(i, n))
-        rows.append((out[0][i].data_ptr(), out[1][i].data_ptr(), m.data_ptr(), v.data_ptr(),
-                     mq.data_ptr(), vq.data_ptr(), n, 0))
+    columns = [map(torch.Tensor.data_ptr, x) for x in list(out) + moments]
+    columns += [map(torch.Tensor.numel, exp_avgs), itertools.repeat(0)]
     with torch.cuda.device(dev):
-        _ext.adamw_values(_ext.adamw_table(rows), torch.cuda.current_stream(dev).cuda_stream)
+        _ext.adamw_values(columns, count, torch.cuda.current_stream(dev).cuda_stream)
     return tuple(out)
 
 
@@ -182,14 +207,21 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
-        # (torch casts floating-point state to the parameter's type; the moments and scales are
-        # float32 whatever that is, and are taken from the given state again)
+        # torch casts the state to the parameter's type; moments, codes and scales keep theirs and
+        # the parameter's order in memory
         given = [i for g in state_dict["param_groups"] for i in g["params"]]
         held = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(given, held):
             for key, t in state_dict["state"].get(i, {}).items():
-                if torch.is_tensor(t) and t.dtype == torch.float32:
+                if not torch.is_tensor(t):
+                    continue
+                if t.shape != p.shape or t.dim() < 2:
                     self.state[p][key] = t.to(device=p.device, copy=True)
+                    continue
+                if t.dtype is not torch.float32 and t.stride() != p.stride():
+                    raise ValueError("8-bit moments of a parameter with the strides {} do not fit "
+                                     "one with {}".format(t.stride(), p.stride()))
+                self.state[p][key] = torch.empty_like(p, dtype=t.dtype).copy_(t)
 
     def _init(self, p, bits):
         s = self.state[p]
