@@ -8,9 +8,9 @@
 // both projections, so activation and product happen in registers and neither projection goes
 // through memory (a training step keeps a and b, in the rows' type, for the backward pass); up to
 // kFewRows rows a kernel that streams the weights once.  Backward: one pass makes da and db, side
-// by side along k and once more transposed, then one product gives dx (k runs over both
-// projections' columns) and one gives both weight gradients (k runs over the rows, cut into
-// slices where there are few tiles; slices are added in order).
+// by side, then one product gives dx (k runs over both projections' columns) and one gives both
+// weight gradients (k runs over the rows, cut into slices where there are few tiles; slices are
+// added in order).
 // 16-bit elements: matrix-bound for many rows, bound by the weights' bytes for few.
 #include "gated_gemm.h"
 
@@ -72,86 +72,69 @@ __global__ void __launch_bounds__(256)
   put_chunk<T>(dst + (r * Split<T>::PARTS) * padded + c, padded, v);
 }
 
-constexpr int kT = 64;  // edge of the tiles that are transposed
-// Writes a tile t[row][col] (kT x kT, in LDS) transposed: columns c0 .. of dst [cols][PARTS][ld],
-// rows r0 ... as its k; `padded` bounds k (a multiple of 8), `cols` the columns.
-template <typename T>
-__device__ __forceinline__ void put_transposed(const float (*t)[kT + 1], int64_t r0, int64_t padded,
-                                               int64_t c0, int64_t cols, int64_t ld,
-                                               typename Split<T>::P *__restrict__ dst) {
-  for (int i = threadIdx.x; i < kT * (kT / 8); i += 256) {
-    const int c = i / (kT / 8), r = i % (kT / 8) * 8;
-    if (c0 + c >= cols || r0 + r >= padded) continue;
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = t[r + e][c];
-    put_chunk<T>(dst + (c0 + c) * Split<T>::PARTS * ld + r0 + r, ld, v);
-  }
-}
-
-// src [rows, cols] -> dst [cols][PARTS][ld], k = rows at `offset`; blockIdx.z: two sources whose
-// rows lie side by side (offset, 2 offset).
-template <typename T>
-__global__ void __launch_bounds__(256)
-    pack_transposed_kernel(const T *__restrict__ src0, const T *__restrict__ src1, int64_t rows,
-                           int64_t cols, int64_t padded, int64_t ld,
-                           typename Split<T>::P *__restrict__ dst) {
-  __shared__ float t[kT][kT + 1];
-  const T *src = blockIdx.z == 0 ? src0 : src1;
-  dst += blockIdx.z * padded;
-  const int64_t r0 = (int64_t)blockIdx.x * kT, c0 = (int64_t)blockIdx.y * kT;
-  const int c = threadIdx.x & 63;
-  for (int r = threadIdx.x >> 6; r < kT; r += 4)
-    t[r][c] = r0 + r < rows && c0 + c < cols ? (float)src[(r0 + r) * cols + c0 + c] : 0.f;
-  __syncthreads();
-  put_transposed<T>(t, r0, padded, c0, cols, ld, dst);
-}
-
-// da and db of a tile of 64 rows x 64 hidden columns.
-//   g  [m][PARTS][2 hp]: da at k = 0 .., db at k = hp ..  (NULL: not wanted)
-//   gt [2 h][PARTS][mp]: rows 0 .. of da, h .. of db      (NULL: not wanted)
-//   sums [tiles of rows][2 h]: column sums of the tile    (NULL: not wanted)
-template <typename T>
+// da and db, rounded (in parts): g [m][PARTS][2 hp], da at 0 .., db at hp .., zeros behind h; and the
+// column sums of every kGradRows rows, sums [tiles of rows][2 h] (NULL: not wanted).  8
+// neighbouring columns of a row to a thread; ALIGNED: rows begin at 16 bytes.  HBM-bound.
+constexpr int kGradRows = 64, kGradAcross = 32;  // rows of a workgroup, threads side by side
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256)
     gated_grad_kernel(const T *__restrict__ dy, const T *__restrict__ a, const T *__restrict__ b,
-                      int64_t m, int64_t h, int act, int64_t hp, int64_t mp,
-                      typename Split<T>::P *__restrict__ g, typename Split<T>::P *__restrict__ gt,
+                      int64_t m, int64_t h, int act, int64_t hp, typename Split<T>::P *__restrict__ g,
                       float *__restrict__ sums) {
-  __shared__ float ta[kT][kT + 1], tb[kT][kT + 1];
-  const int64_t r0 = (int64_t)blockIdx.x * kT, c0 = (int64_t)blockIdx.y * kT;
-  const int c = threadIdx.x & 63;
-  for (int r = threadIdx.x >> 6; r < kT; r += 4) {
-    float da = 0.f, db = 0.f;
-    if (r0 + r < m && c0 + c < h) {
-      const int64_t at = (r0 + r) * h + c0 + c;
-      const float y = (float)dy[at], av = (float)a[at], bv = (float)b[at];
-      float f, d;
-      activate_slope<1>(act, &av, &f, &d);
-      db = y * f;
-      da = y * bv * d;
-    }
-    ta[r][c] = da;
-    tb[r][c] = db;
-  }
-  __syncthreads();
-  if (sums != nullptr && threadIdx.x < 128) {
-    const float (*t)[kT + 1] = threadIdx.x < 64 ? ta : tb;
-    float s = 0.f;
-    for (int r = 0; r < kT; ++r) s += t[r][c];
-    if (c0 + c < h) sums[(int64_t)blockIdx.x * 2 * h + (threadIdx.x < 64 ? 0 : h) + c0 + c] = s;
-  }
-  if (g != nullptr)
-    for (int i = threadIdx.x; i < 2 * kT * (kT / 8); i += 256) {
-      const int which = i / (kT * (kT / 8)), r = i / (kT / 8) % kT, k = i % (kT / 8) * 8;
-      if (r0 + r >= m || c0 + k >= hp) continue;
-      float v[8];
+  constexpr int kDown = 256 / kGradAcross;
+  __shared__ float lds[kDown][kGradAcross * 8 + 1];
+  const int cx = threadIdx.x % kGradAcross, row = threadIdx.x / kGradAcross;
+  const int64_t c = ((int64_t)blockIdx.y * kGradAcross + cx) * 8, r0 = (int64_t)blockIdx.x * kGradRows;
+  float sa[8], sb[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = which == 0 ? ta[r][k + e] : tb[r][k + e];
-      put_chunk<T>(g + (r0 + r) * Split<T>::PARTS * 2 * hp + which * hp + c0 + k, 2 * hp, v);
+  for (int i = 0; i < 8; ++i) sa[i] = sb[i] = 0.f;
+  if (c < hp) {
+#pragma unroll 2
+    for (int64_t r = r0 + row; r < r0 + kGradRows; r += kDown) {
+      if (r >= m) break;
+      float yv[8], av[8], bv[8], f[8], d[8];
+      const int64_t at = r * h + c;
+      if (ALIGNED && c < h) {
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 8; i += V) {
+          load_floats<T, V>(dy + at + i, yv + i);
+          load_floats<T, V>(a + at + i, av + i);
+          load_floats<T, V>(b + at + i, bv + i);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool in = c + i < h;
+          yv[i] = in ? (float)dy[at + i] : 0.f;
+          av[i] = in ? (float)a[at + i] : 0.f;
+          bv[i] = in ? (float)b[at + i] : 0.f;
+        }
+      }
+      activate_slope<8>(act, av, f, d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        av[i] = yv[i] * bv[i] * d[i];
+        bv[i] = yv[i] * f[i];
+        sa[i] += av[i];
+        sb[i] += bv[i];
+      }
+      put_chunk<T>(g + r * Split<T>::PARTS * 2 * hp + c, 2 * hp, av);
+      put_chunk<T>(g + r * Split<T>::PARTS * 2 * hp + hp + c, 2 * hp, bv);
     }
-  if (gt != nullptr) {
-    put_transposed<T>(ta, r0, mp, c0, h, mp, gt);
-    put_transposed<T>(tb, r0, mp, c0, h, mp, gt + h * Split<T>::PARTS * mp);
+  }
+  if (sums == nullptr) return;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lds[row][cx * 8 + i] = which == 0 ? sa[i] : sb[i];
+    __syncthreads();
+    const int64_t col = (int64_t)blockIdx.y * kGradAcross * 8 + threadIdx.x;
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < kDown; ++r) s += lds[r][threadIdx.x];
+    if (col < h) sums[(int64_t)blockIdx.x * 2 * h + which * h + col] = s;
   }
 }
 
@@ -250,11 +233,11 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmArgs g) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int64_t col = n0 + r < g.n ? n0 + r : g.n - 1;
-  const T *wg = static_cast<const T *>(g.b) + col * g.ldb, *wu = static_cast<const T *>(g.b2) + col * g.ldb;
+  const T *wg = static_cast<const T *>(g.b.p) + col * g.b.ld, *wu = static_cast<const T *>(g.b.q) + col * g.b.ld;
   const T *x[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
-    x[t] = static_cast<const T *>(g.a) + (t * 16 + r < g.m ? t * 16 + r : g.m - 1) * g.lda;
+    x[t] = static_cast<const T *>(g.a.p) + (t * 16 + r < g.m ? t * 16 + r : g.m - 1) * g.a.ld;
   f32x4 acc[2 * MT];
 #pragma unroll
   for (int t = 0; t < 2 * MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -367,41 +350,40 @@ template <typename T> int slices_for(const Shape &s) {
                 : z == 1 ? slices_of<typename Tiles<T>::Middle>(s) : slices_of<typename Tiles<T>::Small>(s);
 }
 
-template <typename C, int EPI, typename O>
+template <typename C, bool TA, bool TB, int EPI, typename O>
 int launch(GemmArgs g, int64_t n_tile, int slices, hipStream_t s) {
   g.tiles_m = (int32_t)ceil_div(g.m, C::BM);
   g.tiles_n = (int32_t)ceil_div(n_tile, C::BN);
   SSC_CHECK((int64_t)g.tiles_m * g.tiles_n <= 0x7FFFFFFF, SSC_EINVAL, "too many tiles");
   g.kslice = (int32_t)(ceil_div(ceil_div(g.k, C::BK), slices) * C::BK);
-  hipLaunchKernelGGL((gemm_kernel<C, EPI, O>), dim3(g.tiles_m * g.tiles_n, 1, slices), dim3(C::kThreads),
+  hipLaunchKernelGGL((gemm_kernel<C, TA, TB, EPI, O>), dim3(g.tiles_m * g.tiles_n, 1, slices), dim3(C::kThreads),
                      0, s, g);
   SSC_LAUNCH_CHECK("gated feed-forward product");
   return SSC_OK;
 }
 
-// A product whose result goes to out / out2 (rows from split on), in slices where that pays.
-template <typename T>
+// A product whose result goes to out and out2 (rows from `second` on), in slices where that pays.
+template <typename T, bool TA, bool TB>
 int product(GemmArgs g, float *part, hipStream_t s) {
   const Shape shape = {g.m, g.n, g.k};
   const int size = size_of<T>(shape, true), slices = slices_for<T>(shape);
   typedef Tiles<T> S;
   if (slices == 1) {
-    g.wide = (g.ldo * sizeof(T)) % 16 == 0 && at16(g.out) && (g.out2 == nullptr || at16(g.out2));
-    return size == 2 ? launch<typename S::Large, kStore, T>(g, g.n, 1, s)
-                     : size == 1 ? launch<typename S::Middle, kStore, T>(g, g.n, 1, s)
-                                 : launch<typename S::Small, kStore, T>(g, g.n, 1, s);
+    g.wide = (g.ldo * sizeof(T)) % 16 == 0 && at16(g.out) && at16(g.out2);
+    return size == 2 ? launch<typename S::Large, TA, TB, kStore, T>(g, g.n, 1, s)
+                     : size == 1 ? launch<typename S::Middle, TA, TB, kStore, T>(g, g.n, 1, s)
+                                 : launch<typename S::Small, TA, TB, kStore, T>(g, g.n, 1, s);
   }
   GemmArgs p = g;
   p.out = part;
   p.wide = g.ldo % 4 == 0;
-  const int rc = size == 2 ? launch<typename S::Large, kPartial, float>(p, g.n, slices, s)
-                           : size == 1 ? launch<typename S::Middle, kPartial, float>(p, g.n, slices, s)
-                                       : launch<typename S::Small, kPartial, float>(p, g.n, slices, s);
+  const int rc = size == 2 ? launch<typename S::Large, TA, TB, kPartial, float>(p, g.n, slices, s)
+                           : size == 1 ? launch<typename S::Middle, TA, TB, kPartial, float>(p, g.n, slices, s)
+                                       : launch<typename S::Small, TA, TB, kPartial, float>(p, g.n, slices, s);
   if (rc != SSC_OK) return rc;
-  const int64_t count = g.m * g.n;
+  const int64_t split = g.each * g.n, count = g.second < g.m ? 2 * split : split;
   hipLaunchKernelGGL(add_slices_kernel<T>, dim3((uint32_t)ceil_div(count, 256)), dim3(256), 0, s, part,
-                     slices, count, g.out2 ? g.split * g.n : count, static_cast<T *>(g.out),
-                     static_cast<T *>(g.out2));
+                     slices, count, split, static_cast<T *>(g.out), static_cast<T *>(g.out2));
   SSC_LAUNCH_CHECK("add_slices_kernel");
   return SSC_OK;
 }
@@ -428,10 +410,40 @@ size_t packed_bytes(int64_t rows, int64_t padded, int parts) {
   return align_up((size_t)rows * padded * parts * 2);
 }
 
+// x and the weights as the matrix kernel reads them: as they are, or laid out anew in ws.
+template <typename T> struct Rows {
+  typedef typename Split<T>::P P;
+  static constexpr int PARTS = Split<T>::PARTS;
+  Operand x, wg, wu;
+  static size_t bytes(const Problem &p) {
+    const int64_t kp = up8(p.k);
+    return packed_bytes(p.m, kp, PARTS) + 2 * packed_bytes(p.h, kp, PARTS);
+  }
+  int make(const Problem &p, const void *x0, const void *wg0, const void *wu0, Carver &c, hipStream_t s) {
+    const int64_t kp = up8(p.k);
+    if (reads_plain<T>(p.k, x0, wg0, wu0)) {
+      x.p = x0;
+      wg.p = wg0;
+      wu.p = wu0;
+    } else {
+      P *xp = c.take<P>(p.m * kp * PARTS), *gp = c.take<P>(p.h * kp * PARTS), *up = c.take<P>(p.h * kp * PARTS);
+      int rc = pack_rows<T>(x0, p.m, p.k, kp, xp, s);
+      if (rc == SSC_OK) rc = pack_rows<T>(wg0, p.h, p.k, kp, gp, s);
+      if (rc == SSC_OK) rc = pack_rows<T>(wu0, p.h, p.k, kp, up, s);
+      if (rc != SSC_OK) return rc;
+      x.p = xp;
+      wg.p = gp;
+      wu.p = up;
+    }
+    x.ld = wg.ld = wu.ld = kp * PARTS;
+    x.part = wg.part = wu.part = (int32_t)kp;
+    x.second = wg.second = wu.second = 0x7FFFFFFF;
+    return SSC_OK;
+  }
+};
+
 template <typename T> size_t forward_bytes(const Problem &p) {
-  if (p.m <= kFewRows) return 256;
-  const int64_t kp = up8(p.k);
-  return packed_bytes(p.m, kp, Split<T>::PARTS) + 2 * packed_bytes(p.h, kp, Split<T>::PARTS);
+  return p.m <= kFewRows ? 256 : Rows<T>::bytes(p);
 }
 
 template <typename T, bool ALIGNED> void few_rows(const GemmArgs &g, hipStream_t s) {
@@ -454,125 +466,124 @@ int forward(const Problem &p, const void *x, const void *wg, const void *wu, con
   g.pre_b = b;
   g.ldo = p.h;
   if (p.m <= kFewRows) {
-    g.a = x;
-    g.b = wg;
-    g.b2 = wu;
+    g.a.p = x;
+    g.b.p = wg;
+    g.b.q = wu;
     g.k = (int32_t)p.k;
-    g.lda = g.ldb = p.k;
+    g.a.ld = g.b.ld = p.k;
     const bool aligned = (p.k * sizeof(T)) % 16 == 0 && at16(x) && at16(wg) && at16(wu);
     if (aligned) few_rows<T, true>(g, s);
     else few_rows<T, false>(g, s);
     SSC_LAUNCH_CHECK("few_rows_kernel");
     return SSC_OK;
   }
-  const int64_t kp = up8(p.k);
-  g.k = (int32_t)kp;
-  g.lda = g.ldb = kp * Split<T>::PARTS;
-  if (reads_plain<T>(p.k, x, wg, wu)) {
-    g.a = x;
-    g.b = wg;
-    g.b2 = wu;
-  } else {
-    typedef typename Split<T>::P P;
-    Carver c(ws);
-    P *xp = c.take<P>(p.m * g.lda), *gp = c.take<P>(p.h * g.lda), *up = c.take<P>(p.h * g.lda);
-    int rc = pack_rows<T>(x, p.m, p.k, kp, xp, s);
-    if (rc == SSC_OK) rc = pack_rows<T>(wg, p.h, p.k, kp, gp, s);
-    if (rc == SSC_OK) rc = pack_rows<T>(wu, p.h, p.k, kp, up, s);
-    if (rc != SSC_OK) return rc;
-    g.a = xp;
-    g.b = gp;
-    g.b2 = up;
-  }
+  Carver c(ws);
+  Rows<T> rows = {};
+  const int rc = rows.make(p, x, wg, wu, c, s);
+  if (rc != SSC_OK) return rc;
+  g.k = (int32_t)up8(p.k);
+  g.a = rows.x;
+  g.a.rows = p.m;
+  g.b = rows.wg;
+  g.b.q = rows.wu.p;
+  g.b.rows = p.h;
   g.wide = (p.h * sizeof(T)) % 16 == 0 && at16(y) && at16(a) && at16(b);
-  const int size = size_of<T>({p.m, 2 * p.h, kp}, false);
+  const int size = size_of<T>({p.m, 2 * p.h, g.k}, false);
   typedef Tiles<T> S;
-  return size == 2 ? launch<typename S::Large, kGated, T>(g, 2 * p.h, 1, s)
-                   : size == 1 ? launch<typename S::Middle, kGated, T>(g, 2 * p.h, 1, s)
-                               : launch<typename S::Small, kGated, T>(g, 2 * p.h, 1, s);
+  return size == 2 ? launch<typename S::Large, false, false, kGated, T>(g, 2 * p.h, 1, s)
+                   : size == 1 ? launch<typename S::Middle, false, false, kGated, T>(g, 2 * p.h, 1, s)
+                               : launch<typename S::Small, false, false, kGated, T>(g, 2 * p.h, 1, s);
 }
 
 template <typename T> struct Backward {
   typedef typename Split<T>::P P;
   static constexpr int PARTS = Split<T>::PARTS;
-  int64_t hp, mp;
-  P *g, *gt, *wt, *xt;
+  int64_t hp;  // columns of da and of db in g: a multiple of every tile's k
+  P *g;
   float *sums, *part;
-  size_t bytes;
+  size_t used;
   Backward(const Problem &p, void *ws) {
-    hp = up8(p.h);
-    mp = up8(p.m);
+    hp = ceil_div(p.h, 64) * 64;
     Carver c(ws);
     g = c.take<P>(p.m * PARTS * 2 * hp);
-    gt = c.take<P>(2 * p.h * PARTS * mp);
-    wt = c.take<P>(p.k * PARTS * 2 * hp);
-    xt = c.take<P>(p.k * PARTS * mp);
-    sums = c.take<float>(ceil_div(p.m, kT) * 2 * p.h);
+    sums = c.take<float>(ceil_div(p.m, kGradRows) * 2 * p.h);
     // the slices of the two products, one after the other
-    const Shape sx = {p.m, p.k, 2 * hp}, sw = {2 * p.h, p.k, mp};
-    const int zx = slices_for<T>(sx), zw = slices_for<T>(sw);
+    const int zx = slices_for<T>(dx_shape(p)), zw = slices_for<T>(dw_shape(p));
     const int64_t px = zx > 1 ? zx * p.m * p.k : 0, pw = zw > 1 ? zw * 2 * p.h * p.k : 0;
     part = c.take<float>(px > pw ? px : pw);
-    bytes = c.used;
+    used = c.used;
   }
+  Shape dx_shape(const Problem &p) const { return {p.m, p.k, 2 * hp}; }
+  Shape dw_shape(const Problem &p) const { return {2 * hp, p.k, p.m}; }
+  static size_t bytes(const Problem &p) { return Backward(p, nullptr).used + Rows<T>::bytes(p); }
 };
 
 template <typename T>
 int backward(const Problem &p, const void *x, const void *wg, const void *wu, int act, const void *a,
              const void *b, const void *dy, void *dx, void *dwg, void *dwu, void *dbg, void *dbu,
              void *ws, hipStream_t s) {
-  typedef typename Split<T>::P P;
   constexpr int PARTS = Split<T>::PARTS;
   const Backward<T> w(p, ws);
-  const bool weights = dwg != nullptr, biases = dbg != nullptr || dbu != nullptr;
-  const dim3 tiles((uint32_t)ceil_div(p.m, kT), (uint32_t)ceil_div(p.h, kT));
-  hipLaunchKernelGGL(gated_grad_kernel<T>, tiles, dim3(256), 0, s, static_cast<const T *>(dy),
-                     static_cast<const T *>(a), static_cast<const T *>(b), p.m, p.h, act, w.hp, w.mp,
-                     dx ? w.g : nullptr, weights ? w.gt : nullptr, biases ? w.sums : nullptr);
+  const bool biases = dbg != nullptr || dbu != nullptr;
+  const dim3 tiles((uint32_t)ceil_div(p.m, kGradRows), (uint32_t)ceil_div(w.hp, kGradAcross * 8));
+  const bool aligned = (p.h % 8) == 0 && at16(dy) && at16(a) && at16(b);
+#define SSC_GRAD(ALIGNED)                                                                              \
+  hipLaunchKernelGGL((gated_grad_kernel<T, ALIGNED>), tiles, dim3(256), 0, s, static_cast<const T *>(dy), \
+                     static_cast<const T *>(a), static_cast<const T *>(b), p.m, p.h, act, w.hp, w.g,   \
+                     biases ? w.sums : nullptr)
+  if (aligned) SSC_GRAD(true);
+  else SSC_GRAD(false);
+#undef SSC_GRAD
   SSC_LAUNCH_CHECK("gated_grad_kernel");
   if (biases) {
     hipLaunchKernelGGL(bias_grad_kernel<T>, dim3((uint32_t)ceil_div(2 * p.h, 16)), dim3(256), 0, s, w.sums,
-                       ceil_div(p.m, kT), p.h, static_cast<T *>(dbg), static_cast<T *>(dbu));
+                       ceil_div(p.m, kGradRows), p.h, static_cast<T *>(dbg), static_cast<T *>(dbu));
     SSC_LAUNCH_CHECK("bias_grad_kernel");
   }
+  if (dx == nullptr && dwg == nullptr) return SSC_OK;
+  Carver c(static_cast<char *>(ws) + w.used);
+  Rows<T> rows = {};
+  int rc = rows.make(p, x, wg, wu, c, s);
+  if (rc != SSC_OK) return rc;
+  Operand grad = {};
+  grad.p = w.g;
+  grad.ld = PARTS * 2 * w.hp;
+  grad.part = (int32_t)(2 * w.hp);
+  grad.second = 0x7FFFFFFF;
   GemmArgs g = {};
+  g.n = p.k;
+  g.ldo = p.k;
   if (dx) {
-    hipLaunchKernelGGL(pack_transposed_kernel<T>,
-                       dim3((uint32_t)ceil_div(p.h, kT), (uint32_t)ceil_div(p.k, kT), 2), dim3(256), 0, s,
-                       static_cast<const T *>(wg), static_cast<const T *>(wu), p.h, p.k, w.hp, 2 * w.hp,
-                       w.wt);
-    SSC_LAUNCH_CHECK("pack_transposed_kernel");
-    g.a = w.g;
-    g.b = w.wt;
+    g.a = grad;
+    g.a.rows = p.m;
+    g.b = rows.wg;
+    g.b.q = rows.wu.p;
+    g.b.rows = up8(p.k);
+    g.b.second = (int32_t)w.hp;
+    g.b.deep = (int32_t)p.h;
     g.m = p.m;
-    g.n = p.k;
     g.k = (int32_t)(2 * w.hp);
-    g.lda = g.ldb = PARTS * 2 * w.hp;
     g.out = dx;
-    g.split = p.m;
-    g.ldo = p.k;
-    const int rc = product<T>(g, w.part, s);
+    g.second = g.each = p.m;
+    rc = product<T, false, true>(g, w.part, s);
     if (rc != SSC_OK) return rc;
   }
-  if (weights) {
-    hipLaunchKernelGGL(pack_transposed_kernel<T>,
-                       dim3((uint32_t)ceil_div(p.m, kT), (uint32_t)ceil_div(p.k, kT), 1), dim3(256), 0, s,
-                       static_cast<const T *>(x), static_cast<const T *>(x), p.m, p.k, w.mp, w.mp, w.xt);
-    SSC_LAUNCH_CHECK("pack_transposed_kernel");
-    g.a = w.gt;
-    g.b = w.xt;
-    g.m = 2 * p.h;
-    g.n = p.k;
-    g.k = (int32_t)w.mp;
-    g.lda = g.ldb = PARTS * w.mp;
+  if (dwg) {
+    g.a = grad;
+    g.a.rows = 2 * w.hp;
+    g.a.deep = (int32_t)p.m;
+    g.b = rows.x;
+    g.b.rows = up8(p.k);
+    g.b.deep = (int32_t)p.m;
+    g.m = 2 * w.hp;
+    g.k = (int32_t)p.m;
     g.out = dwg;
     g.out2 = dwu;
-    g.split = p.h;
-    g.ldo = p.k;
-    const int rc = product<T>(g, w.part, s);
-    if (rc != SSC_OK) return rc;
+    g.second = w.hp;
+    g.each = p.h;
+    rc = product<T, true, true>(g, w.part, s);
   }
-  return SSC_OK;
+  return rc;
 }
 
 // What 32-bit offsets inside a few rows allow.
@@ -620,7 +631,7 @@ extern "C" int ssc_gated_fwd(int32_t dtype, const void *x, int64_t m, int64_t k,
 extern "C" size_t ssc_gated_bwd_workspace_bytes(int32_t dtype, int64_t m, int64_t k, int64_t h) {
   if (m <= 0) return 256;
   const Problem p = {m, k, h};
-  return dtype == SSC_F32 ? Backward<float>(p, nullptr).bytes : Backward<f16>(p, nullptr).bytes;
+  return dtype == SSC_F32 ? Backward<float>::bytes(p) : Backward<f16>::bytes(p);
 }
 
 extern "C" int ssc_gated_bwd(int32_t dtype, const void *x, int64_t m, int64_t k, const void *w_gate,

@@ -1,12 +1,14 @@
-// The matrix product behind the gated feed-forward block:
+// The matrix products behind the gated feed-forward block:
 //
 //   C[m, n] = sum over k of A[m, k] B[n, k]
 //
-// on 16-bit matrix instructions, both operands with k running along memory.  float operands come
-// as three bfloat16 parts a = a0 + a1 + a2 (each the rounding of what the parts before it leave:
-// 24 bits in all), laid one behind another in a row, and six of the nine products of parts are
-// taken: a0 b0, a0 b1, a1 b0, a1 b1, a0 b2, a2 b0.  What is left out is below 2^-24 of |a||b|,
-// and bfloat16 has the exponents of float, so no scaling is needed.
+// on 16-bit matrix instructions.  An operand lies in memory either with k along its rows or as
+// the transpose, with k down the columns; LDS reads that transpose blocks of 4 x 16 elements
+// give the matrix instruction the same registers from either, so nothing is ever laid out anew.
+// float operands come as three bfloat16 parts a = a0 + a1 + a2 (each the rounding of what the
+// parts before it leave: 24 bits in all), laid one behind another in a row, and six of the nine
+// products of parts are taken: a0 b0, a0 b1, a1 b0, a1 b1, a0 b2, a2 b0.  What is left out is
+// below 2^-23 of |a||b|, and bfloat16 has the exponents of float, so no scaling is needed.
 #ifndef SSC_GATED_GEMM_H_
 #define SSC_GATED_GEMM_H_
 
@@ -17,7 +19,7 @@ namespace ssc {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -36,17 +38,26 @@ enum Epilogue {
   kPartial,  // C as float into the slice blockIdx.z of a workspace
 };
 
+// An operand: `rows` rows (m or n) along k.
+//   k along its rows:  p[row * ld + k], with a second array (kGated) for every other run of rows
+//   k down its columns: p[k * ld + row], and from k = `second` on q[(k - second) * ld + row];
+//                       each array has `deep` values of k, the rest count as zero
+// Parts (float operands) lie `part` elements apart.
+struct Operand {
+  const void *p, *q;
+  int64_t rows, ld;
+  int32_t part, deep, second;
+};
+
 struct GemmArgs {
-  const void *a;          // [m, lda] 16-bit elements
-  const void *b, *b2;     // [n, ldb]; kGated: w_gate and w_up, [n / 2, ldb] each
-  int64_t m, n;           // kGated: n counts the hidden columns
-  int64_t lda, ldb;       // elements of a row (all parts)
-  int32_t k;              // elements along k of one part, a multiple of 8
-  int32_t kslice;         // elements along k of a slice (kPartial), a multiple of the tile's
+  Operand a, b;
+  int64_t m, n;           // of the results; kGated: n counts the hidden columns
+  int32_t k;              // a multiple of 8 (k along rows), of the tile's (k down columns)
+  int32_t kslice;         // values of k in a slice (kPartial), a multiple of the tile's
   int32_t tiles_m, tiles_n;
-  void *out, *out2;       // kStore: rows from `split` on go to out2
-  int64_t split;
-  int64_t ldo;
+  // kStore, kPartial: rows from `second` on are those of out2; out and out2 have `each` rows
+  void *out, *out2;
+  int64_t second, each, ldo;
   void *pre_a, *pre_b;    // kGated: a and b [m, n], or NULL
   const void *bias_a, *bias_b;
   int32_t act;
@@ -58,8 +69,6 @@ template <typename T_, int PARTS_, int BM_, int BN_, int BK_, int WM_, int WN_> 
   typedef T_ T;
   static constexpr int PARTS = PARTS_, BM = BM_, BN = BN_, BK = BK_, WM = WM_, WN = WN_;
   static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
-  static constexpr int kChunks = BK / 8;                     // 16-byte chunks of a row
-  static constexpr int kRowsAtOnce = 64 / kChunks;           // rows one load of a wave covers
   static constexpr int kABytes = BM * BK * 2, kBBytes = BN * BK * 2;
   static constexpr int kStage = (kABytes + kBBytes) * PARTS;
   static constexpr int kMi = BM / WM / 16, kNi = BN / WN / 16;
@@ -67,16 +76,8 @@ template <typename T_, int PARTS_, int BM_, int BN_, int BK_, int WM_, int WN_> 
   static constexpr int kPitch = kNi * 16 + 4;
   static constexpr int kTurn = kWaves * 64 * kPitch * 4;
   static constexpr int kLds = 2 * kStage > kTurn ? 2 * kStage : kTurn;
-  static constexpr int kALoads = BM / (kRowsAtOnce * kWaves), kBLoads = BN / (kRowsAtOnce * kWaves);
-  static_assert(kALoads * kRowsAtOnce * kWaves == BM && kBLoads * kRowsAtOnce * kWaves == BN, "tile");
   static_assert((BK == 64 || BK == 32) && kMi % 4 == 0 && kNi % 2 == 0, "tile");
 };
-
-// The 16-byte chunk c of row r lies at chunk c ^ swizzle(r) of the row's place in LDS: the 16
-// rows that a matrix operand's lanes read at the same c then fall on all banks evenly.
-template <int BK> __device__ __forceinline__ int swizzle(int r) {
-  return BK == 64 ? (r & 7) : ((r >> 1) & 3);
-}
 
 // Workgroups go to the 8 dies in turn; each die gets a run of tiles that are neighbours, in
 // strips of 8 tiles along m, so that its level-2 cache serves their common rows.
@@ -92,14 +93,118 @@ __device__ __forceinline__ void tile_of(const GemmArgs &g, int &tm, int &tn) {
 }
 
 typedef __attribute__((address_space(3))) void *lds_ptr;
+typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
 typedef decltype(__builtin_amdgcn_make_buffer_rsrc((void *)0, (short)0, 0, 0)) rsrc_t;
 
-template <typename C>
+// One operand's tile: R rows x BK values of k, loaded by W waves straight into LDS, and read back
+// as the 16 x 32 blocks of the matrix instruction (lane: row lane & 15, k = 8 (lane >> 4) ...).
+//
+// k along rows: a tile's row is BK elements; chunk c (16 bytes) of row r lies at chunk
+// c ^ swizzle(r), so that the 16 rows which are read at the same c fall on all banks evenly.
+template <int R, int BK, int W, bool TR> struct Side {
+  static constexpr int kChunks = BK / 8, kRows = 64 / kChunks;  // rows that a load of a wave covers
+  static constexpr int kLoads = R / (kRows * W);
+  static_assert(kLoads * kRows * W == R, "tile");
+  rsrc_t rs[kLoads];
+  int off, kc;
+
+  static __device__ __forceinline__ int swizzle(int r) { return BK == 64 ? (r & 7) : ((r >> 1) & 3); }
+
+  // A resource for every load of a wave: it spans the few rows of that load, so offsets stay small
+  // however long the rows are, and rows behind the matrix read as zero.  HALF > 0: runs of HALF
+  // rows come from p and q in turn.
+  template <int HALF>
+  __device__ __forceinline__ void init(const Operand &o, int64_t r0, int w, int lane) {
+    const int srow = lane / kChunks;
+    kc = ((lane % kChunks) ^ swizzle(srow)) * 8;  // (a load begins at a multiple of 8 rows)
+    off = (int)((srow * o.ld + kc) * 2);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int first = (i * W + w) * kRows;
+      const bool other = HALF > 0 && first % (2 * HALF) >= HALF;
+      const int64_t row = r0 + (HALF > 0 ? first / (2 * HALF) * HALF + first % HALF : first);
+      const int64_t rows = o.rows - row < kRows ? o.rows - row : kRows;
+      rs[i] = __builtin_amdgcn_make_buffer_rsrc(
+          (void *)((const char *)(other ? o.q : o.p) + (rows > 0 ? row : 0) * o.ld * 2), 0,
+          rows > 0 ? (int)(rows * o.ld * 2) : 0, 0x00020000);
+    }
+  }
+  __device__ __forceinline__ void load(const Operand &, int k0, int k_end, int skip, int w, char *to) {
+    const int o = k0 + kc < k_end ? off : 0x7FFFFFFF;  // (what lies behind the slice counts as zero)
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs[i], (lds_ptr)(to + (i * W + w) * 1024), 16, o,
+                                               (k0 + skip) * 2, 0, 0);
+  }
+  template <typename F>
+  static __device__ __forceinline__ F block(const char *tile, int row0, int kk, int lane) {
+    const int r = lane & 15, c = (kk * 4 + (lane >> 4)) ^ swizzle(r);
+    return *reinterpret_cast<const F *>(tile + (row0 + r) * (BK * 2) + (c << 4));
+  }
+};
+
+// k down columns: the tile's rows are those of memory, R elements for each k; an LDS read takes 4
+// elements of one k from each of 16 lanes and hands every lane the 4 values of k of one column, so
+// two reads make a block's 8.  The lanes of a read touch 4 neighbouring k (of 16 k in all) at 32
+// neighbouring bytes: chunk c of row k lies at c ^ swizzle(k), which spreads them over the banks.
+template <int R, int BK, int W> struct Side<R, BK, W, true> {
+  static constexpr int kChunks = R / 8, kRows = 64 / kChunks;  // k that a load of a wave covers
+  static constexpr int kLoads = BK / (kRows * W);
+  static_assert(kLoads * kRows * W == BK && kChunks >= 8, "tile");
+  const char *base, *base2;
+  int off[kLoads], step;
+
+  static __device__ __forceinline__ int swizzle(int k) {
+    return R >= 128 ? ((k & 3) | (k >> 1 & 4)) << 1 : (k & 3) << 1;
+  }
+
+  template <int HALF>
+  __device__ __forceinline__ void init(const Operand &o, int64_t r0, int w, int lane) {
+    base = (const char *)o.p + r0 * 2;
+    base2 = (const char *)o.q + r0 * 2;
+    step = (int)(o.ld - r0 < 0x3FFFFFFF ? o.ld - r0 : 0x3FFFFFFF) * 2;  // bytes left in a row
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int k = (i * W + w) * kRows + lane / kChunks;
+      const int c = ((lane % kChunks) ^ swizzle(k)) * 8;
+      // (columns behind the matrix count as zero)
+      off[i] = r0 + c < o.rows ? (int)((k * o.ld + c) * 2) : 0x7FFFFFFF;
+    }
+  }
+  __device__ __forceinline__ void load(const Operand &o, int k0, int, int skip, int w, char *to) {
+    const bool other = k0 >= o.second;
+    const int64_t k = other ? k0 - o.second : k0;
+    const int64_t left = o.deep - k < BK ? o.deep - k : BK;  // values of k that exist
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)((other ? base2 : base) + (left > 0 ? k * o.ld * 2 : 0)), 0,
+        left > 0 ? (int)((left - 1) * o.ld * 2) + step : 0, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(to + (i * W + w) * 1024), 16, off[i],
+                                               skip * 2, 0, 0);
+  }
+  template <typename F>
+  static __device__ __forceinline__ F block(const char *tile, int row0, int kk, int lane) {
+    const int q = lane >> 4, l = lane & 15;
+    s16x4 v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = kk * 32 + q * 8 + h * 4 + (l >> 2);
+      const int col = row0 + (l & 3) * 4;
+      v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(
+          tile + k * (R * 2) + (((col >> 3) ^ swizzle(k)) << 4) + (col & 4) * 2));
+    }
+    return __builtin_bit_cast(F, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// (`stage` is not written while it is read: without __restrict__ every read would wait for the
+// loads to the other stage)
+template <typename C, typename SA, typename SB>
 __device__ __forceinline__ void gemm_compute(const char *__restrict__ stage, int wm, int wn,
                                              f32x4 (&acc)[C::kNi][C::kMi]) {
   typedef typename Frag<typename C::T>::type F;
-  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  constexpr int kRow = C::BK * 2;
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int kk = 0; kk < C::BK / 32; ++kk) {
     F a[C::PARTS][C::kMi], b[C::PARTS][C::kNi];
@@ -107,15 +212,11 @@ __device__ __forceinline__ void gemm_compute(const char *__restrict__ stage, int
     for (int p = 0; p < C::PARTS; ++p) {
       const char *sa = stage + p * C::kABytes, *sb = stage + C::PARTS * C::kABytes + p * C::kBBytes;
 #pragma unroll
-      for (int j = 0; j < C::kNi; ++j) {
-        const int row = wn * (C::kNi * 16) + j * 16 + r;
-        b[p][j] = *reinterpret_cast<const F *>(sb + row * kRow + (((kk * 4 + q) ^ swizzle<C::BK>(r)) << 4));
-      }
+      for (int j = 0; j < C::kNi; ++j)
+        b[p][j] = SB::template block<F>(sb, wn * (C::kNi * 16) + j * 16, kk, lane);
 #pragma unroll
-      for (int i = 0; i < C::kMi; ++i) {
-        const int row = wm * (C::kMi * 16) + i * 16 + r;
-        a[p][i] = *reinterpret_cast<const F *>(sa + row * kRow + (((kk * 4 + q) ^ swizzle<C::BK>(r)) << 4));
-      }
+      for (int i = 0; i < C::kMi; ++i)
+        a[p][i] = SA::template block<F>(sa, wm * (C::kMi * 16) + i * 16, kk, lane);
     }
 #pragma unroll
     for (int i = 0; i < C::kMi; ++i)
@@ -155,8 +256,8 @@ __device__ __forceinline__ void load_turned(const float *p, float *v) {
   *reinterpret_cast<f32x4 *>(v + 4) = *reinterpret_cast<const f32x4 *>(p + 4);
 }
 
-// O: type of the outputs.
-template <typename C, int EPI, typename O>
+// TA, TB: whether A and B have k down their columns.  O: type of the outputs.
+template <typename C, bool TA, bool TB, int EPI, typename O>
 __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
 #ifdef __HIP_DEVICE_COMPILE__  // (loads to LDS are no builtins of the host's compiler)
   __shared__ __align__(1024) char lds[C::kLds];
@@ -171,51 +272,20 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
   constexpr int kCols = EPI == kGated ? C::BN / 2 : C::BN;
   constexpr int kHalf = C::kNi * 8;
   const int64_t n0 = (int64_t)tn * kCols;
-
-  // A resource for every load of a wave: it spans the few rows of that load, so offsets stay
-  // small however long the rows are, and rows behind the matrix read as zero.
-  const int srow = lane / C::kChunks;                       // row of a load of the wave
-  const int kc = ((lane % C::kChunks) ^ swizzle<C::BK>(srow)) * 8;  // (a load begins at a multiple of 8 rows)
-  const int va = (int)((srow * g.lda + kc) * 2), vb = (int)((srow * g.ldb + kc) * 2);
-  rsrc_t rsa[C::kALoads], rsb[C::kBLoads];
-#pragma unroll
-  for (int i = 0; i < C::kALoads; ++i) {
-    const int64_t row = m0 + (i * C::kWaves + w) * C::kRowsAtOnce;
-    const int64_t rows = g.m - row < C::kRowsAtOnce ? g.m - row : C::kRowsAtOnce;
-    rsa[i] = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)((const char *)g.a + (rows > 0 ? row : 0) * g.lda * 2), 0,
-        rows > 0 ? (int)(rows * g.lda * 2) : 0, 0x00020000);
-  }
-#pragma unroll
-  for (int i = 0; i < C::kBLoads; ++i) {
-    const int first = (i * C::kWaves + w) * C::kRowsAtOnce;
-    const bool up = EPI == kGated && first % (2 * kHalf) >= kHalf;
-    const int64_t row = n0 + (EPI == kGated ? first / (2 * kHalf) * kHalf + first % kHalf : first);
-    const int64_t rows = g.n - row < C::kRowsAtOnce ? g.n - row : C::kRowsAtOnce;
-    rsb[i] = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)((const char *)(up ? g.b2 : g.b) + (rows > 0 ? row : 0) * g.ldb * 2), 0,
-        rows > 0 ? (int)(rows * g.ldb * 2) : 0, 0x00020000);
-  }
+  typedef Side<C::BM, C::BK, C::kWaves, TA> SA;
+  typedef Side<C::BN, C::BK, C::kWaves, TB> SB;
+  SA sa;
+  SB sb;
+  sa.template init<0>(g.a, m0, w, lane);
+  sb.template init<EPI == kGated ? kHalf : 0>(g.b, n0, w, lane);
   const int k_begin = EPI == kPartial ? (int)blockIdx.z * g.kslice : 0;
   const int k_end = EPI == kPartial && k_begin + g.kslice < g.k ? k_begin + g.kslice : g.k;
-
   auto issue = [&](int k0, int s) {
     char *st = lds + s * C::kStage;
-    const bool in = k0 + kc < k_end;  // (what lies behind the slice counts as zero)
-    const int oa = in ? va : 0x7FFFFFFF, ob = in ? vb : 0x7FFFFFFF;
 #pragma unroll
     for (int p = 0; p < C::PARTS; ++p) {
-      const int at = (k0 + p * g.k) * 2;
-#pragma unroll
-      for (int i = 0; i < C::kALoads; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rsa[i], (lds_ptr)(st + p * C::kABytes + (i * C::kWaves + w) * 1024), 16, oa, at, 0, 0);
-#pragma unroll
-      for (int i = 0; i < C::kBLoads; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rsb[i],
-            (lds_ptr)(st + C::PARTS * C::kABytes + p * C::kBBytes + (i * C::kWaves + w) * 1024), 16,
-            ob, at, 0, 0);
+      sa.load(g.a, k0, k_end, p * g.a.part, w, st + p * C::kABytes);
+      sb.load(g.b, k0, k_end, p * g.b.part, w, st + C::PARTS * C::kABytes + p * C::kBBytes);
     }
   };
 
@@ -231,7 +301,7 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
   for (int k0 = k_begin; k0 < k_end; k0 += C::BK, s ^= 1) {
     __syncthreads();
     if (k0 + C::BK < k_end) issue(k0 + C::BK, s ^ 1);
-    gemm_compute<C>(lds + s * C::kStage, wm, wn, acc);
+    gemm_compute<C, SA, SB>(lds + s * C::kStage, wm, wn, acc);
   }
   __syncthreads();
 
@@ -277,10 +347,12 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
           for (int e = 0; e < 8; ++e) f[e] *= b[e];
           store_row<O>(static_cast<O *>(g.out) + row * g.ldo + col, f, left, wide);
         } else {
-          O *y;
-          if (EPI == kPartial) y = static_cast<O *>(g.out) + ((int64_t)blockIdx.z * g.m + row) * g.ldo;
-          else if (row >= g.split) y = static_cast<O *>(g.out2) + (row - g.split) * g.ldo;
-          else y = static_cast<O *>(g.out) + row * g.ldo;
+          const bool other = row >= g.second;
+          const int64_t r2 = other ? row - g.second : row;
+          if (r2 >= g.each) continue;
+          O *y;  // (a slice's rows: those of out and of out2, one behind the other)
+          if (EPI == kPartial) y = static_cast<O *>(g.out) + ((blockIdx.z * (g.second < g.m ? 2 : 1) + (other ? 1 : 0)) * g.each + r2) * g.ldo;
+          else y = static_cast<O *>(other ? g.out2 : g.out) + r2 * g.ldo;
           store_row<O>(y + col, a, left, wide);
         }
       }
