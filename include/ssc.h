@@ -933,23 +933,23 @@ int ssc_groupnorm_bwd(int32_t dtype, const void *x, const void *dy /* [n,c] */, 
 
 /* Both projections of a gated feed-forward block, the activation and the product:
  *   a = x w_gate^T + b_gate,  b = x w_up^T + b_up,  y = act(a) * b
- * x [m,k], weights [h,k], biases [h] (each may be NULL), y, a, b [m,h], all of type dtype and
- * contiguous.  a and b (both or none NULL) are what the backward pass reads; they are rounded to
- * dtype, y is computed from the sums before that.  Products of float elements are taken in parts
- * (six bfloat16 products, 24 bits), sums are float.
+ * x [m,k], weights [h,k], biases [h] (each may be NULL), y [m,h], all of type dtype and contiguous.
+ * kept (ssc_gated_kept_bytes, at 16 bytes; NULL where no backward pass follows): a and b for the
+ * backward pass, in 24 bits for 16-bit types and in 32 for floats.  Products of float elements are
+ * taken in parts (six bfloat16 products, 24 bits), sums are float; a float infinity in x or the
+ * weights comes out as NaN (infinity times a part that is zero).
  * ssc_gated_bwd: dx [m,k], dw_gate, dw_up [h,k] (both or none), db_gate, db_up [h], each NULL
- * where it is not wanted.  With m = 0 nothing is written.  m <= 2^24, k and h <= 2^21.
- * A float infinity in x or the weights comes out as NaN (infinity times a part that is zero). */
+ * where it is not wanted.  With m = 0 nothing is written.  m <= 2^24, k and h <= 2^21. */
 size_t ssc_gated_fwd_workspace_bytes(int32_t dtype, int64_t m, int64_t k, int64_t h);
+size_t ssc_gated_kept_bytes(int32_t dtype, int64_t m, int64_t h);
 int ssc_gated_fwd(int32_t dtype, const void *x, int64_t m, int64_t k, const void *w_gate,
                   const void *w_up, int64_t h, const void *b_gate, const void *b_up, int32_t act,
-                  void *y, void *a, void *b, void *workspace, size_t workspace_bytes,
-                  ssc_stream_t stream);
+                  void *y, void *kept, void *workspace, size_t workspace_bytes, ssc_stream_t stream);
 size_t ssc_gated_bwd_workspace_bytes(int32_t dtype, int64_t m, int64_t k, int64_t h);
 int ssc_gated_bwd(int32_t dtype, const void *x, int64_t m, int64_t k, const void *w_gate,
-                  const void *w_up, int64_t h, int32_t act, const void *a, const void *b,
-                  const void *dy, void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up,
-                  void *workspace, size_t workspace_bytes, ssc_stream_t stream);
+                  const void *w_up, int64_t h, int32_t act, const void *kept, const void *dy, void *dx,
+                  void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *workspace,
+                  size_t workspace_bytes, ssc_stream_t stream);
 
 /* One AdamW step over n_tensors tensors (host array), each updated in place:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,

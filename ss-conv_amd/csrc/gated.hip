@@ -6,7 +6,7 @@
 //
 // Forward: one launch of the matrix kernel (gated_gemm.h) whose tiles hold the same columns of
 // both projections, so activation and product happen in registers and neither projection goes
-// through memory (a training step keeps a and b, in the rows' type, for the backward pass); up to
+// through memory (a training step keeps a and b, in 24 or 32 bits, for the backward pass); up to
 // kFewRows rows a kernel that streams the weights once.  Backward: one pass makes da and db, side
 // by side, then one product gives dx (k runs over both projections' columns) and one gives both
 // weight gradients (k runs over the rows, cut into slices where there are few tiles; slices are
@@ -78,9 +78,9 @@ __global__ void __launch_bounds__(256)
 constexpr int kGradRows = 64, kGradAcross = 32;  // rows of a workgroup, threads side by side
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256)
-    gated_grad_kernel(const T *__restrict__ dy, const T *__restrict__ a, const T *__restrict__ b,
-                      int64_t m, int64_t h, int act, int64_t hp, typename Split<T>::P *__restrict__ g,
-                      float *__restrict__ sums) {
+    gated_grad_kernel(const T *__restrict__ dy, const void *__restrict__ ab, int64_t m, int64_t h, int act,
+                      int64_t hp, typename Split<T>::P *__restrict__ g, float *__restrict__ sums) {
+  const Kept<T> kept(ab, m, h);
   constexpr int kDown = 256 / kGradAcross;
   __shared__ float lds[kDown][kGradAcross * 8 + 1];
   const int cx = threadIdx.x % kGradAcross, row = threadIdx.x / kGradAcross;
@@ -97,19 +97,14 @@ __global__ void __launch_bounds__(256)
       if (ALIGNED && c < h) {
         constexpr int V = 16 / sizeof(T);
 #pragma unroll
-        for (int i = 0; i < 8; i += V) {
-          load_floats<T, V>(dy + at + i, yv + i);
-          load_floats<T, V>(a + at + i, av + i);
-          load_floats<T, V>(b + at + i, bv + i);
-        }
+        for (int i = 0; i < 8; i += V) load_floats<T, V>(dy + at + i, yv + i);
+        kept.template get<true>(0, at, 8, av);
+        kept.template get<true>(1, at, 8, bv);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const bool in = c + i < h;
-          yv[i] = in ? (float)dy[at + i] : 0.f;
-          av[i] = in ? (float)a[at + i] : 0.f;
-          bv[i] = in ? (float)b[at + i] : 0.f;
-        }
+        for (int i = 0; i < 8; ++i) yv[i] = c + i < h ? (float)dy[at + i] : 0.f;
+        kept.template get<false>(0, at, h - c, av);
+        kept.template get<false>(1, at, h - c, bv);
       }
       activate_slope<8>(act, av, f, d);
 #pragma unroll
@@ -293,9 +288,10 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmArgs g) {
     if (c0 + e < g.n) {
       const int64_t at = row * g.ldo + c0 + e;
       static_cast<T *>(g.out)[at] = (T)(f[e] * b[e]);
-      if (g.pre_a) {
-        static_cast<T *>(g.pre_a)[at] = (T)a[e];
-        static_cast<T *>(g.pre_b)[at] = (T)b[e];
+      if (g.kept) {
+        const Kept<T> kept(g.kept, g.m, g.n);
+        kept.put(0, at, a + e, 1, false);
+        kept.put(1, at, b + e, 1, false);
       }
     }
 }
@@ -454,7 +450,7 @@ template <typename T, bool ALIGNED> void few_rows(const GemmArgs &g, hipStream_t
 
 template <typename T>
 int forward(const Problem &p, const void *x, const void *wg, const void *wu, const void *bg,
-            const void *bu, int act, void *y, void *a, void *b, void *ws, hipStream_t s) {
+            const void *bu, int act, void *y, void *kept, void *ws, hipStream_t s) {
   GemmArgs g = {};
   g.m = p.m;
   g.n = p.h;
@@ -462,8 +458,7 @@ int forward(const Problem &p, const void *x, const void *wg, const void *wu, con
   g.bias_b = bu;
   g.act = act;
   g.out = y;
-  g.pre_a = a;
-  g.pre_b = b;
+  g.kept = kept;
   g.ldo = p.h;
   if (p.m <= kFewRows) {
     g.a.p = x;
@@ -487,7 +482,7 @@ int forward(const Problem &p, const void *x, const void *wg, const void *wu, con
   g.b = rows.wg;
   g.b.q = rows.wu.p;
   g.b.rows = p.h;
-  g.wide = (p.h * sizeof(T)) % 16 == 0 && at16(y) && at16(a) && at16(b);
+  g.wide = (p.h * sizeof(T)) % 16 == 0 && at16(y);
   const int size = size_of<T>({p.m, 2 * p.h, g.k}, false);
   typedef Tiles<T> S;
   return size == 2 ? launch<typename S::Large, false, false, kGated, T>(g, 2 * p.h, 1, s)
@@ -519,17 +514,17 @@ template <typename T> struct Backward {
 };
 
 template <typename T>
-int backward(const Problem &p, const void *x, const void *wg, const void *wu, int act, const void *a,
-             const void *b, const void *dy, void *dx, void *dwg, void *dwu, void *dbg, void *dbu,
+int backward(const Problem &p, const void *x, const void *wg, const void *wu, int act, const void *kept,
+             const void *dy, void *dx, void *dwg, void *dwu, void *dbg, void *dbu,
              void *ws, hipStream_t s) {
   constexpr int PARTS = Split<T>::PARTS;
   const Backward<T> w(p, ws);
   const bool biases = dbg != nullptr || dbu != nullptr;
   const dim3 tiles((uint32_t)ceil_div(p.m, kGradRows), (uint32_t)ceil_div(w.hp, kGradAcross * 8));
-  const bool aligned = (p.h % 8) == 0 && at16(dy) && at16(a) && at16(b);
+  const bool aligned = (p.h % 8) == 0 && at16(dy);
 #define SSC_GRAD(ALIGNED)                                                                              \
   hipLaunchKernelGGL((gated_grad_kernel<T, ALIGNED>), tiles, dim3(256), 0, s, static_cast<const T *>(dy), \
-                     static_cast<const T *>(a), static_cast<const T *>(b), p.m, p.h, act, w.hp, w.g,   \
+                     kept, p.m, p.h, act, w.hp, w.g,   \
                      biases ? w.sums : nullptr)
   if (aligned) SSC_GRAD(true);
   else SSC_GRAD(false);
@@ -610,22 +605,28 @@ extern "C" size_t ssc_gated_fwd_workspace_bytes(int32_t dtype, int64_t m, int64_
   return dtype == SSC_F32 ? forward_bytes<float>(p) : forward_bytes<f16>(p);
 }
 
+extern "C" size_t ssc_gated_kept_bytes(int32_t dtype, int64_t m, int64_t h) {
+  const size_t bytes = dtype == SSC_F32 ? Kept<float>::bytes(m, h) : Kept<f16>::bytes(m, h);
+  return bytes > 0 ? bytes : 16;
+}
+
 extern "C" int ssc_gated_fwd(int32_t dtype, const void *x, int64_t m, int64_t k, const void *w_gate,
                              const void *w_up, int64_t h, const void *b_gate, const void *b_up,
-                             int32_t act, void *y, void *a, void *b, void *ws, size_t ws_bytes,
+                             int32_t act, void *y, void *kept, void *ws, size_t ws_bytes,
                              ssc_stream_t stream) {
   const int rc = check(dtype, m, k, h, act);
   if (rc != SSC_OK) return rc;
   if (m == 0) return SSC_OK;
-  SSC_CHECK(x && w_gate && w_up && y && (a == nullptr) == (b == nullptr), SSC_EINVAL, "NULL pointer");
+  SSC_CHECK(x && w_gate && w_up && y, SSC_EINVAL, "NULL pointer");
+  SSC_CHECK(at16(kept), SSC_EINVAL, "what is kept begins at 16 bytes");
   SSC_CHECK(ws != nullptr && ws_bytes >= ssc_gated_fwd_workspace_bytes(dtype, m, k, h), SSC_EWORKSPACE,
             "workspace of %zu bytes, %zu are needed", ws_bytes,
             ssc_gated_fwd_workspace_bytes(dtype, m, k, h));
   const Problem p = {m, k, h};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == SSC_F32) return forward<float>(p, x, w_gate, w_up, b_gate, b_up, act, y, a, b, ws, s);
-  if (dtype == SSC_F16) return forward<f16>(p, x, w_gate, w_up, b_gate, b_up, act, y, a, b, ws, s);
-  return forward<bf16>(p, x, w_gate, w_up, b_gate, b_up, act, y, a, b, ws, s);
+  if (dtype == SSC_F32) return forward<float>(p, x, w_gate, w_up, b_gate, b_up, act, y, kept, ws, s);
+  if (dtype == SSC_F16) return forward<f16>(p, x, w_gate, w_up, b_gate, b_up, act, y, kept, ws, s);
+  return forward<bf16>(p, x, w_gate, w_up, b_gate, b_up, act, y, kept, ws, s);
 }
 
 extern "C" size_t ssc_gated_bwd_workspace_bytes(int32_t dtype, int64_t m, int64_t k, int64_t h) {
@@ -635,21 +636,22 @@ extern "C" size_t ssc_gated_bwd_workspace_bytes(int32_t dtype, int64_t m, int64_
 }
 
 extern "C" int ssc_gated_bwd(int32_t dtype, const void *x, int64_t m, int64_t k, const void *w_gate,
-                             const void *w_up, int64_t h, int32_t act, const void *a, const void *b,
-                             const void *dy, void *dx, void *dw_gate, void *dw_up, void *db_gate,
-                             void *db_up, void *ws, size_t ws_bytes, ssc_stream_t stream) {
+                             const void *w_up, int64_t h, int32_t act, const void *kept, const void *dy,
+                             void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *ws,
+                             size_t ws_bytes, ssc_stream_t stream) {
   const int rc = check(dtype, m, k, h, act);
   if (rc != SSC_OK) return rc;
   if (m == 0) return SSC_OK;
-  SSC_CHECK(x && w_gate && w_up && a && b && dy && (dw_gate == nullptr) == (dw_up == nullptr), SSC_EINVAL,
+  SSC_CHECK(x && w_gate && w_up && kept && dy && (dw_gate == nullptr) == (dw_up == nullptr), SSC_EINVAL,
             "NULL pointer");
+  SSC_CHECK(at16(kept), SSC_EINVAL, "what is kept begins at 16 bytes");
   SSC_CHECK(ws != nullptr && ws_bytes >= ssc_gated_bwd_workspace_bytes(dtype, m, k, h), SSC_EWORKSPACE,
             "workspace of %zu bytes, %zu are needed", ws_bytes,
             ssc_gated_bwd_workspace_bytes(dtype, m, k, h));
   const Problem p = {m, k, h};
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define SSC_GATED_BWD(T) \
-  backward<T>(p, x, w_gate, w_up, act, a, b, dy, dx, dw_gate, dw_up, db_gate, db_up, ws, s)
+  backward<T>(p, x, w_gate, w_up, act, kept, dy, dx, dw_gate, dw_up, db_gate, db_up, ws, s)
   return dtype == SSC_F32 ? SSC_GATED_BWD(float) : dtype == SSC_F16 ? SSC_GATED_BWD(f16) : SSC_GATED_BWD(bf16);
 #undef SSC_GATED_BWD
 }

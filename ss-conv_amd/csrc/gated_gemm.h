@@ -33,7 +33,7 @@ template <> struct Frag<bf16> { typedef bf16x8 type; };
 
 // What is done with the product.
 enum Epilogue {
-  kGated,    // rows of B are w_gate and w_up: y = act(a + b_gate) * (b + b_up), optionally a and b
+  kGated,    // rows of B are w_gate and w_up: y = act(a + b_gate) * (b + b_up), optionally a and b kept
   kStore,    // C rounded to the output type
   kPartial,  // C as float into the slice blockIdx.z of a workspace
 };
@@ -58,7 +58,7 @@ struct GemmArgs {
   // kStore, kPartial: rows from `second` on are those of out2; out and out2 have `each` rows
   void *out, *out2;
   int64_t second, each, ldo;
-  void *pre_a, *pre_b;    // kGated: a and b [m, n], or NULL
+  void *kept;             // kGated: a and b for the backward pass (Kept), or NULL
   const void *bias_a, *bias_b;
   int32_t act;
   int32_t wide;           // rows and pointers of the outputs allow stores of 16 bytes
@@ -80,14 +80,14 @@ template <typename T_, int PARTS_, int BM_, int BN_, int BK_, int WM_, int WN_> 
 };
 
 // Workgroups go to the 8 dies in turn; each die gets a run of tiles that are neighbours, in
-// strips of 8 tiles along m, so that its level-2 cache serves their common rows.
+// strips of 4 tiles along m, so that its level-2 cache serves their common rows.
 __device__ __forceinline__ void tile_of(const GemmArgs &g, int &tm, int &tn) {
   const int total = g.tiles_m * g.tiles_n, id = blockIdx.x;
   const int die = id & 7, each = total >> 3, more = total & 7;
   const int at = die * each + (die < more ? die : more) + (id >> 3);
-  const int strip = at / (8 * g.tiles_n), first = strip * 8;
-  const int wide = g.tiles_m - first < 8 ? g.tiles_m - first : 8;
-  const int in = at - strip * 8 * g.tiles_n;
+  const int strip = at / (4 * g.tiles_n), first = strip * 4;
+  const int wide = g.tiles_m - first < 4 ? g.tiles_m - first : 4;
+  const int in = at - strip * 4 * g.tiles_n;
   tm = first + in % wide;
   tn = in / wide;
 }
@@ -114,7 +114,7 @@ template <int R, int BK, int W, bool TR> struct Side {
   // however long the rows are, and rows behind the matrix read as zero.  HALF > 0: runs of HALF
   // rows come from p and q in turn.
   template <int HALF>
-  __device__ __forceinline__ void init(const Operand &o, int64_t r0, int w, int lane) {
+  __device__ __forceinline__ void init(const Operand &o, int64_t r0, int, int w, int lane) {
     const int srow = lane / kChunks;
     kc = ((lane % kChunks) ^ swizzle(srow)) * 8;  // (a load begins at a multiple of 8 rows)
     off = (int)((srow * o.ld + kc) * 2);
@@ -129,6 +129,7 @@ template <int R, int BK, int W, bool TR> struct Side {
           rows > 0 ? (int)(rows * o.ld * 2) : 0, 0x00020000);
     }
   }
+  template <bool LAST>
   __device__ __forceinline__ void load(const Operand &, int k0, int k_end, int skip, int w, char *to) {
     const int o = k0 + kc < k_end ? off : 0x7FFFFFFF;  // (what lies behind the slice counts as zero)
 #pragma unroll
@@ -151,37 +152,47 @@ template <int R, int BK, int W> struct Side<R, BK, W, true> {
   static constexpr int kChunks = R / 8, kRows = 64 / kChunks;  // k that a load of a wave covers
   static constexpr int kLoads = BK / (kRows * W);
   static_assert(kLoads * kRows * W == BK && kChunks >= 8, "tile");
-  const char *base, *base2;
-  int off[kLoads], step;
+  const char *cur, *next;  // where the next step's first value of k lies; the second array
+  int64_t left;            // values of k that cur's array has left
+  int k, off[kLoads], row, rest;  // row: bytes of a row, rest: of the last one
 
   static __device__ __forceinline__ int swizzle(int k) {
     return R >= 128 ? ((k & 3) | (k >> 1 & 4)) << 1 : (k & 3) << 1;
   }
 
   template <int HALF>
-  __device__ __forceinline__ void init(const Operand &o, int64_t r0, int w, int lane) {
-    base = (const char *)o.p + r0 * 2;
-    base2 = (const char *)o.q + r0 * 2;
-    step = (int)(o.ld - r0 < 0x3FFFFFFF ? o.ld - r0 : 0x3FFFFFFF) * 2;  // bytes left in a row
+  __device__ __forceinline__ void init(const Operand &o, int64_t r0, int k_begin, int w, int lane) {
+    const bool other = k_begin >= o.second;
+    k = k_begin;
+    left = o.deep - (other ? k_begin - o.second : k_begin);
+    next = (const char *)o.q + r0 * 2;
+    cur = (other ? next : (const char *)o.p + r0 * 2) + (o.deep - left) * o.ld * 2;
+    row = (int)o.ld * 2;
+    rest = (int)(o.ld - r0) * 2;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int k = (i * W + w) * kRows + lane / kChunks;
-      const int c = ((lane % kChunks) ^ swizzle(k)) * 8;
+      const int kr = (i * W + w) * kRows + lane / kChunks;
+      const int c = ((lane % kChunks) ^ swizzle(kr)) * 8;
       // (columns behind the matrix count as zero)
-      off[i] = r0 + c < o.rows ? (int)((k * o.ld + c) * 2) : 0x7FFFFFFF;
+      off[i] = r0 + c < o.rows ? kr * row + c * 2 : 0x7FFFFFFF;
     }
   }
-  __device__ __forceinline__ void load(const Operand &o, int k0, int, int skip, int w, char *to) {
-    const bool other = k0 >= o.second;
-    const int64_t k = other ? k0 - o.second : k0;
-    const int64_t left = o.deep - k < BK ? o.deep - k : BK;  // values of k that exist
-    const auto rs = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)((other ? base2 : base) + (left > 0 ? k * o.ld * 2 : 0)), 0,
-        left > 0 ? (int)((left - 1) * o.ld * 2) + step : 0, 0x00020000);
+  // One part of the next BK values of k; with the last part the step is done.
+  template <bool LAST>
+  __device__ __forceinline__ void load(const Operand &o, int, int, int skip, int w, char *to) {
+    const int there = left < BK ? (int)left : BK;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)cur, 0,
+                                                      there > 0 ? (there - 1) * row + rest : 0, 0x00020000);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(to + (i * W + w) * 1024), 16, off[i],
                                                skip * 2, 0, 0);
+    if constexpr (LAST) {
+      k += BK;
+      const bool turn = k == o.second;
+      cur = turn ? next : cur + (int64_t)BK * row;
+      left = turn ? (int64_t)o.deep : left - BK;
+    }
   }
   template <typename F>
   static __device__ __forceinline__ F block(const char *tile, int row0, int kk, int lane) {
@@ -198,40 +209,56 @@ template <int R, int BK, int W> struct Side<R, BK, W, true> {
   }
 };
 
-// (`stage` is not written while it is read: without __restrict__ every read would wait for the
-// loads to the other stage)
-template <typename C, typename SA, typename SB>
-__device__ __forceinline__ void gemm_compute(const char *__restrict__ stage, int wm, int wn,
-                                             f32x4 (&acc)[C::kNi][C::kMi]) {
+template <typename C> struct Blocks {
   typedef typename Frag<typename C::T>::type F;
+  F a[C::PARTS][C::kMi], b[C::PARTS][C::kNi];
+};
+
+// The blocks of 32 values of k that a wave multiplies next.  (`stage` is not written while it is
+// read: without __restrict__ every read would wait for the loads to the other stage.)
+template <typename C, typename SA, typename SB>
+__device__ __forceinline__ void read_blocks(const char *__restrict__ stage, int kk, int wm, int wn,
+                                            Blocks<C> &x) {
+  typedef typename Blocks<C>::F F;
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int kk = 0; kk < C::BK / 32; ++kk) {
-    F a[C::PARTS][C::kMi], b[C::PARTS][C::kNi];
+  for (int p = 0; p < C::PARTS; ++p) {
+    const char *sa = stage + p * C::kABytes, *sb = stage + C::PARTS * C::kABytes + p * C::kBBytes;
 #pragma unroll
-    for (int p = 0; p < C::PARTS; ++p) {
-      const char *sa = stage + p * C::kABytes, *sb = stage + C::PARTS * C::kABytes + p * C::kBBytes;
-#pragma unroll
-      for (int j = 0; j < C::kNi; ++j)
-        b[p][j] = SB::template block<F>(sb, wn * (C::kNi * 16) + j * 16, kk, lane);
-#pragma unroll
-      for (int i = 0; i < C::kMi; ++i)
-        a[p][i] = SA::template block<F>(sa, wm * (C::kMi * 16) + i * 16, kk, lane);
-    }
+    for (int j = 0; j < C::kNi; ++j)
+      x.b[p][j] = SB::template block<F>(sb, wn * (C::kNi * 16) + j * 16, kk, lane);
 #pragma unroll
     for (int i = 0; i < C::kMi; ++i)
-#pragma unroll
-      for (int j = 0; j < C::kNi; ++j) {
-        if constexpr (C::PARTS == 3) {
-          acc[j][i] = mfma16(b[2][j], a[0][i], acc[j][i]);
-          acc[j][i] = mfma16(b[0][j], a[2][i], acc[j][i]);
-          acc[j][i] = mfma16(b[1][j], a[1][i], acc[j][i]);
-          acc[j][i] = mfma16(b[1][j], a[0][i], acc[j][i]);
-          acc[j][i] = mfma16(b[0][j], a[1][i], acc[j][i]);
-        }
-        acc[j][i] = mfma16(b[0][j], a[0][i], acc[j][i]);
-      }
+      x.a[p][i] = SA::template block<F>(sa, wm * (C::kMi * 16) + i * 16, kk, lane);
   }
+}
+
+template <typename C>
+__device__ __forceinline__ void multiply(const Blocks<C> &x, f32x4 (&acc)[C::kNi][C::kMi]) {
+#pragma unroll
+  for (int i = 0; i < C::kMi; ++i)
+#pragma unroll
+    for (int j = 0; j < C::kNi; ++j) {
+      if constexpr (C::PARTS == 3) {
+        acc[j][i] = mfma16(x.b[2][j], x.a[0][i], acc[j][i]);
+        acc[j][i] = mfma16(x.b[0][j], x.a[2][i], acc[j][i]);
+        acc[j][i] = mfma16(x.b[1][j], x.a[1][i], acc[j][i]);
+        acc[j][i] = mfma16(x.b[1][j], x.a[0][i], acc[j][i]);
+        acc[j][i] = mfma16(x.b[0][j], x.a[1][i], acc[j][i]);
+      }
+      acc[j][i] = mfma16(x.b[0][j], x.a[0][i], acc[j][i]);
+    }
+}
+
+// One LDS read behind every few matrix instructions, so that both units are busy all the time.
+template <int READS, int MULS> __device__ __forceinline__ void interleave() {
+  constexpr int kEach = MULS / READS > 0 ? MULS / READS : 1;
+#pragma unroll
+  for (int i = 0; i < READS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);  // matrix instructions
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);    // an LDS read
+  }
+  __builtin_amdgcn_sched_group_barrier(0x8, MULS, 0);
 }
 
 // 8 neighbouring results of a row, of which `left` exist.
@@ -250,6 +277,79 @@ __device__ __forceinline__ void store_row(O *p, const float *v, int64_t left, bo
       if (i < left) p[i] = (O)v[i];
   }
 }
+
+// What a training step keeps of the projections a (which 0) and b (1): [m, n] each, 16-bit ones
+// with 8 more bits of the rounding's remainder, in units of 2^-8 of the value's last place.  The
+// backward pass rounds da and db to 16 bits once, as an operand of its products has to be; with
+// a and b rounded as well the gradients would be off by three such roundings instead of two.
+template <typename O> struct Kept {
+  static constexpr bool kMore = sizeof(O) == 2;
+  // remainder / (unit in the last place / 256) = remainder / 2^exponent * kUnits
+  static constexpr float kUnits = __is_same(O, f16) ? 262144.f : 32768.f;
+  O *p;
+  int8_t *q;
+  int64_t count;
+  __host__ __device__ Kept(const void *base, int64_t m, int64_t n)
+      : p(static_cast<O *>(const_cast<void *>(base))), count((m * n + 15) / 16 * 16) {
+    q = reinterpret_cast<int8_t *>(p + 2 * count);
+  }
+  static size_t bytes(int64_t m, int64_t n) {
+    return (size_t)((m * n + 15) / 16 * 16) * 2 * (sizeof(O) + (kMore ? 1 : 0));
+  }
+  static __device__ __forceinline__ uint32_t exponent(O hi) {
+    return __float_as_uint((float)hi) & 0x7F800000u;
+  }
+  static __device__ __forceinline__ int more(float v) {
+    const O hi = (O)v;
+    const uint32_t e = exponent(hi);
+    // (2^-exponent; 0 for the largest exponent, infinities and NaN: nothing more is kept)
+    const float inv = e < 0x7F000000u ? __uint_as_float(0x7F000000u - e) : 0.f;
+    const float r = e < 0x7F000000u ? (v - (float)hi) * inv * kUnits : 0.f;
+    return (int)rintf(fminf(fmaxf(r, -127.f), 127.f));
+  }
+  static __device__ __forceinline__ float value(O hi, int lo) {
+    return (float)hi + (float)lo * (__uint_as_float(exponent(hi) < 0x7F000000u ? exponent(hi) : 0u) * (1.f / kUnits));
+  }
+  __device__ __forceinline__ void put(int which, int64_t at, const float *v, int64_t left, bool wide) const {
+    store_row<O>(p + which * count + at, v, left, wide);
+    if constexpr (kMore) {
+      int8_t *to = q + which * count + at;
+      if (wide && left >= 8) {
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i / 4] |= ((uint32_t)more(v[i]) & 255u) << (i % 4 * 8);
+        *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+      } else {
+        for (int i = 0; i < 8; ++i)
+          if (i < left) to[i] = (int8_t)more(v[i]);
+      }
+    }
+  }
+  // 8 values; ALIGNED: all of them exist and lie at 8 elements.
+  template <bool ALIGNED>
+  __device__ __forceinline__ void get(int which, int64_t at, int64_t left, float *v) const {
+    const O *from = p + which * count + at;
+    if constexpr (!kMore) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        if (ALIGNED) load_floats<O, 4>(from + i, v + i);
+        else
+          for (int e = i; e < i + 4; ++e) v[e] = e < left ? (float)from[e] : 0.f;
+      }
+    } else {
+      const int8_t *more = q + which * count + at;
+      if constexpr (ALIGNED) {
+        const auto hi = *reinterpret_cast<const typename Pack<O, 8>::type *>(from);
+        const uint2 lo = *reinterpret_cast<const uint2 *>(more);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = value(hi[i], (int8_t)((i < 4 ? lo.x : lo.y) >> (i % 4 * 8)));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? value(from[i], more[i]) : 0.f;
+      }
+    }
+  }
+};
 
 __device__ __forceinline__ void load_turned(const float *p, float *v) {
   *reinterpret_cast<f32x4 *>(v) = *reinterpret_cast<const f32x4 *>(p);
@@ -276,17 +376,22 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
   typedef Side<C::BN, C::BK, C::kWaves, TB> SB;
   SA sa;
   SB sb;
-  sa.template init<0>(g.a, m0, w, lane);
-  sb.template init<EPI == kGated ? kHalf : 0>(g.b, n0, w, lane);
   const int k_begin = EPI == kPartial ? (int)blockIdx.z * g.kslice : 0;
   const int k_end = EPI == kPartial && k_begin + g.kslice < g.k ? k_begin + g.kslice : g.k;
+  sa.template init<0>(g.a, m0, k_begin, w, lane);
+  sb.template init<EPI == kGated ? kHalf : 0>(g.b, n0, k_begin, w, lane);
+  // The loads of the step that begins at k0: called for one step after the other.
   auto issue = [&](int k0, int s) {
     char *st = lds + s * C::kStage;
-#pragma unroll
-    for (int p = 0; p < C::PARTS; ++p) {
-      sa.load(g.a, k0, k_end, p * g.a.part, w, st + p * C::kABytes);
-      sb.load(g.b, k0, k_end, p * g.b.part, w, st + C::PARTS * C::kABytes + p * C::kBBytes);
+    if constexpr (C::PARTS == 3) {
+      sa.template load<false>(g.a, k0, k_end, 0, w, st);
+      sb.template load<false>(g.b, k0, k_end, 0, w, st + 3 * C::kABytes);
+      sa.template load<false>(g.a, k0, k_end, g.a.part, w, st + C::kABytes);
+      sb.template load<false>(g.b, k0, k_end, g.b.part, w, st + 3 * C::kABytes + C::kBBytes);
     }
+    sa.template load<true>(g.a, k0, k_end, (C::PARTS - 1) * g.a.part, w, st + (C::PARTS - 1) * C::kABytes);
+    sb.template load<true>(g.b, k0, k_end, (C::PARTS - 1) * g.b.part, w,
+                           st + C::PARTS * C::kABytes + (C::PARTS - 1) * C::kBBytes);
   };
 
   f32x4 acc[C::kNi][C::kMi];
@@ -295,13 +400,40 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
 #pragma unroll
     for (int i = 0; i < C::kMi; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // Two stages: while one is multiplied, the other one's loads are under way.
-  issue(k_begin, 0);
-  int s = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += C::BK, s ^= 1) {
+  if constexpr (C::PARTS == 1) {
+    // Two stages in LDS and two sets of blocks in registers: while one set is multiplied the
+    // next one is read, and a stage is loaded while the other one is read.
+    constexpr int kUnits = C::BK / 32;
+    static_assert(kUnits == 2, "the sets change places once a stage");
+    constexpr int kReads = C::kMi * (TA ? 2 : 1) + C::kNi * (TB ? 2 : 1), kMuls = C::kMi * C::kNi;
+    Blocks<C> x0, x1;
+    issue(k_begin, 0);
     __syncthreads();
-    if (k0 + C::BK < k_end) issue(k0 + C::BK, s ^ 1);
-    gemm_compute<C, SA, SB>(lds + s * C::kStage, wm, wn, acc);
+    issue(k_begin + C::BK, 1);
+    read_blocks<C, SA, SB>(lds, 0, wm, wn, x0);
+    int s = 0;
+    for (int k0 = k_begin; k0 < k_end; k0 += C::BK, s ^= 1) {
+      read_blocks<C, SA, SB>(lds + s * C::kStage, 1, wm, wn, x1);
+      multiply<C>(x0, acc);
+      interleave<kReads, kMuls>();
+      __syncthreads();  // stage s is read, the other one is there
+      if (k0 + 2 * C::BK < k_end) issue(k0 + 2 * C::BK, s);
+      // (behind the last step these are blocks that nobody multiplies)
+      read_blocks<C, SA, SB>(lds + (s ^ 1) * C::kStage, 0, wm, wn, x0);
+      multiply<C>(x1, acc);
+      interleave<kReads, kMuls>();
+    }
+  } else {
+    // Two stages: while one is multiplied, the other one's loads are under way.
+    issue(k_begin, 0);
+    int s = 0;
+    for (int k0 = k_begin; k0 < k_end; k0 += C::BK, s ^= 1) {
+      __syncthreads();
+      if (k0 + C::BK < k_end) issue(k0 + C::BK, s ^ 1);
+      Blocks<C> x;
+      read_blocks<C, SA, SB>(lds + s * C::kStage, 0, wm, wn, x);
+      multiply<C>(x, acc);
+    }
   }
   __syncthreads();
 
@@ -338,9 +470,10 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
             for (int e = 0; e < 8 && e < left; ++e) a[e] += (float)static_cast<const O *>(g.bias_a)[col + e];
           if (g.bias_b != nullptr)
             for (int e = 0; e < 8 && e < left; ++e) b[e] += (float)static_cast<const O *>(g.bias_b)[col + e];
-          if (g.pre_a != nullptr) {
-            store_row<O>(static_cast<O *>(g.pre_a) + row * g.ldo + col, a, left, wide);
-            store_row<O>(static_cast<O *>(g.pre_b) + row * g.ldo + col, b, left, wide);
+          if (g.kept != nullptr) {
+            const Kept<O> kept(g.kept, g.m, g.n);
+            kept.put(0, row * g.n + col, a, left, wide);
+            kept.put(1, row * g.n + col, b, left, wide);
           }
           activate<8>(g.act, a, f);
 #pragma unroll

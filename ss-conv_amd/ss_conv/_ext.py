@@ -188,11 +188,12 @@ _SIGNATURES = {
     "ssc_groupnorm_bwd": (ctypes.c_int, [_i32, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _vp,
                                          _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ssc_gated_fwd_workspace_bytes": (_sz, [_i32, _i64, _i64, _i64]),
+    "ssc_gated_kept_bytes": (_sz, [_i32, _i64, _i64]),
     "ssc_gated_fwd": (ctypes.c_int, [_i32, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _vp,
-                                     _vp, _vp, _sz, _vp]),
+                                     _vp, _sz, _vp]),
     "ssc_gated_bwd_workspace_bytes": (_sz, [_i32, _i64, _i64, _i64]),
     "ssc_gated_bwd": (ctypes.c_int, [_i32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp,
-                                     _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+                                     _vp, _vp, _vp, _vp, _sz, _vp]),
     "ssc_adamw_step": (ctypes.c_int, [_vp, _i32, _i32, _dbl, _dbl, _dbl, _dbl, _dbl, _i64, _vp]),
     "ssc_adamw_values": (ctypes.c_int, [_vp, _i32, _vp]),
 }
@@ -1909,22 +1910,21 @@ def groupnorm_backward(x, dy, offsets, groups, weight, bias, act, mean, rstd, wa
 
 
 def gated_forward(x, w_gate, w_up, b_gate, b_up, act, keep):
-    """y[m, h] of contiguous rows x[m, k]; with `keep` also the projections a, b[m, h] that the
-    backward pass reads (else None)."""
+    """y[m, h] of contiguous rows x[m, k]; with `keep` also what the backward pass reads of both
+    projections (else None)."""
     m, k = x.shape
     h = w_gate.size(0)
     y = x.new_empty((m, h))
-    a = x.new_empty((m, h)) if keep else None
-    b = x.new_empty((m, h)) if keep else None
     elem = ELEM[x.dtype]
+    kept = _workspace(_lib.ssc_gated_kept_bytes(elem, m, h), x.device) if keep else None
     ws = _workspace(_lib.ssc_gated_fwd_workspace_bytes(elem, m, k, h), x.device)
     _check(_lib.ssc_gated_fwd(elem, _ptr(x), m, k, w_gate.data_ptr(), w_up.data_ptr(), h,
-                              _ptr(b_gate), _ptr(b_up), act, _ptr(y), _ptr(a), _ptr(b),
-                              ws.data_ptr(), ws.numel(), _stream(x)))
-    return y, a, b
+                              _ptr(b_gate), _ptr(b_up), act, _ptr(y), _ptr(kept), ws.data_ptr(),
+                              ws.numel(), _stream(x)))
+    return y, kept
 
 
-def gated_backward(x, w_gate, w_up, act, a, b, dy, want):
+def gated_backward(x, w_gate, w_up, act, kept, dy, want):
     """dx, dw_gate, dw_up, db_gate, db_up (None where `want` says so), m >= 1."""
     m, k = x.shape
     h = w_gate.size(0)
@@ -1936,7 +1936,7 @@ def gated_backward(x, w_gate, w_up, act, a, b, dy, want):
     elem = ELEM[x.dtype]
     ws = _workspace(_lib.ssc_gated_bwd_workspace_bytes(elem, m, k, h), x.device)
     _check(_lib.ssc_gated_bwd(elem, x.data_ptr(), m, k, w_gate.data_ptr(), w_up.data_ptr(), h, act,
-                              a.data_ptr(), b.data_ptr(), dy.data_ptr(), _ptr(dx), _ptr(dw_gate),
+                              kept.data_ptr(), dy.data_ptr(), _ptr(dx), _ptr(dw_gate),
                               _ptr(dw_up), _ptr(db_gate), _ptr(db_up), ws.data_ptr(), ws.numel(),
                               _stream(x)))
     return dx, dw_gate if want[1] else None, dw_up if want[2] else None, db_gate, db_up

@@ -4,8 +4,8 @@
 
 Both projections, the activation and the product are one kernel (`ssc_gated_fwd`), the gradients
 come from hand-written kernels too (`ssc_gated_bwd`): float32, float16 and bfloat16, sums in
-float32, one rounding of the result.  A training step keeps both projections, rounded to the
-rows' type, for the backward pass.
+float32, one rounding of the result.  A training step keeps both projections for the backward
+pass, in 24 bits for 16-bit types and in 32 for floats.
 
 A block mixes the channels of a row: use it on scalar (order 0) fields, where that keeps the
 network equivariant.
@@ -23,21 +23,21 @@ from ss_conv import pointwise
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
-        y, a, b = _ext.gated_forward(x, w_gate, w_up, b_gate, b_up, act, True)
-        ctx.save_for_backward(x, w_gate, w_up, a, b)
+        y, kept = _ext.gated_forward(x, w_gate, w_up, b_gate, b_up, act, True)
+        ctx.save_for_backward(x, w_gate, w_up, kept)
         ctx.act = act
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, w_gate, w_up, a, b = ctx.saved_tensors
+        x, w_gate, w_up, kept = ctx.saved_tensors
         want = ctx.needs_input_grad[:5]
         if x.size(0) == 0:
             shapes = (x, w_gate, w_up, w_gate[:, 0], w_gate[:, 0])
             return tuple(torch.zeros_like(t) if w else None for t, w in zip(shapes, want)) + (None,)
         with _ext.on_device_of(x):
-            return _ext.gated_backward(x, w_gate, w_up, ctx.act, a, b, dy.contiguous(), want) + \
+            return _ext.gated_backward(x, w_gate, w_up, ctx.act, kept, dy.contiguous(), want) + \
                 (None,)
 
 

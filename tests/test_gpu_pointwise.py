@@ -10,8 +10,9 @@ and statistics in float32 or more):
         instead of rounding, so 2 (n + 8) 2^-24
   an activation and its slope: exponentials of z are off by (|z| + 4) 2^-23, so is what follows
 
-A 16-bit gradient passes through one more rounding of da and db (and of what the backward pass
-reads), each at most u of the value; the bounds below add them up element by element.
+A 16-bit gradient passes through one more rounding of da and db, at most u of the value; the bounds
+below add up the errors element by element and leave as much again for what the backward pass
+reads.
 """
 import math
 
@@ -774,10 +775,10 @@ def test_pointwise_c_abi_refusals():
     assert norm(n=0, x=None) == 0
     gated = lambda **k: lib.ssc_gated_fwd(*dict(  # noqa: E731
         dict(dtype=0, x=x.data_ptr(), m=4, k=8, wg=x.data_ptr(), wu=x.data_ptr(), h=4, bg=None,
-             bu=None, act=0, y=ws.data_ptr(), a=None, b=None, ws=ws.data_ptr(), bytes=ws.numel(),
+             bu=None, act=0, y=ws.data_ptr(), kept=None, ws=ws.data_ptr(), bytes=ws.numel(),
              stream=None), **k).values())
     assert gated(dtype=5) == gated(k=0) == gated(h=0) == gated(act=6) == gated(m=-1) == \
-        gated(m=2 ** 40) == gated(wg=None) == gated(a=ws.data_ptr()) == _ext.SSC_EINVAL
+        gated(m=2 ** 40) == gated(wg=None) == gated(kept=ws.data_ptr() + 8) == _ext.SSC_EINVAL
     assert gated(bytes=0) == _ext.SSC_EWORKSPACE
     assert gated(m=0, x=None) == 0
     table = _ext.adamw_table([[x.data_ptr()]] + [[0]] * 5 + [[32], [0]])
