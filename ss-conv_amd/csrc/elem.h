@@ -64,6 +64,20 @@ __device__ __forceinline__ void store_floats(T *p, const float *in) {
   }
 }
 
+// The same for results that are not read again soon: they need not push other lines out of the
+// caches.
+template <typename T, int V>
+__device__ __forceinline__ void store_floats_once(T *p, const float *in) {
+  if constexpr (V == 1) {
+    p[0] = (T)in[0];
+  } else {
+    typename Pack<T, V>::type v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (T)in[i];
+    __builtin_nontemporal_store(v, reinterpret_cast<typename Pack<T, V>::type *>(p));
+  }
+}
+
 // Element i of an array whose type is known at run time only (parameter vectors).
 __device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {
   if (dtype == SSC_F32) return static_cast<const float *>(p)[i];

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(256)
       if (ALIGNED && c < h) {
         constexpr int V = 16 / sizeof(T);
 #pragma unroll
-        for (int i = 0; i < 8; i += V) load_floats<T, V>(dy + at + i, yv + i);
+        for (int i = 0; i < 8; i += V) load_floats_once<T, V>(dy + at + i, yv + i);
         kept.template get<true>(0, at, 8, av);
         kept.template get<true>(1, at, 8, bv);
       } else {
@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmArgs g) {
       static_cast<T *>(g.out)[at] = (T)(f[e] * b[e]);
       if (g.kept) {
         const Kept<T> kept(g.kept, g.m, g.n);
-        kept.put(0, at, a + e, 1, false);
-        kept.put(1, at, b + e, 1, false);
+        kept.template put<false>(0, at, a + e, 1, false);
+        kept.template put<false>(1, at, b + e, 1, false);
       }
     }
 }
@@ -302,7 +302,7 @@ bool at16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Tiles: large ones reuse more of what they read, small ones fill the chip where there are few.
 template <typename T> struct Tiles {
-  typedef Tile<T, 1, 256, 256, 64, 2, 4> Large;
+  typedef Tile<T, 1, 256, 256, 64, 4, 2> Large;
   typedef Tile<T, 1, 128, 128, 64, 2, 2> Middle;
   typedef Tile<T, 1, 64, 128, 64, 1, 4> Small;
 };

@@ -72,11 +72,12 @@ template <typename T_, int PARTS_, int BM_, int BN_, int BK_, int WM_, int WN_> 
   static constexpr int kABytes = BM * BK * 2, kBBytes = BN * BK * 2;
   static constexpr int kStage = (kABytes + kBBytes) * PARTS;
   static constexpr int kMi = BM / WM / 16, kNi = BN / WN / 16;
-  // the epilogue turns a wave's results in LDS, 64 rows at a time
+  // the epilogue turns a wave's results in LDS, some rows at a time
   static constexpr int kPitch = kNi * 16 + 4;
-  static constexpr int kTurn = kWaves * 64 * kPitch * 4;
+  static constexpr int kTurnBlocks = kNi > 4 ? 2 : 4, kTurnRows = kTurnBlocks * 16;
+  static constexpr int kTurn = kWaves * kTurnRows * kPitch * 4;
   static constexpr int kLds = 2 * kStage > kTurn ? 2 * kStage : kTurn;
-  static_assert((BK == 64 || BK == 32) && kMi % 4 == 0 && kNi % 2 == 0, "tile");
+  static_assert((BK == 64 || BK == 32) && kMi % kTurnBlocks == 0 && kNi % 2 == 0 && kLds <= 160 * 1024, "tile");
 };
 
 // Workgroups go to the 8 dies in turn; each die gets a run of tiles that are neighbours, in
@@ -261,15 +262,15 @@ template <int READS, int MULS> __device__ __forceinline__ void interleave() {
   __builtin_amdgcn_sched_group_barrier(0x8, MULS, 0);
 }
 
-// 8 neighbouring results of a row, of which `left` exist.
-template <typename O>
+// 8 neighbouring results of a row, of which `left` exist.  ONCE: past the caches.
+template <bool ONCE, typename O>
 __device__ __forceinline__ void store_row(O *p, const float *v, int64_t left, bool wide) {
   if (wide && left >= 8) {
-    if constexpr (sizeof(O) == 4) {
-      store_floats<O, 4>(p, v);
-      store_floats<O, 4>(p + 4, v + 4);
-    } else {
-      store_floats<O, 8>(p, v);
+    constexpr int V = 16 / sizeof(O);
+#pragma unroll
+    for (int i = 0; i < 8; i += V) {
+      if constexpr (ONCE) store_floats_once<O, V>(p + i, v + i);
+      else store_floats<O, V>(p + i, v + i);
     }
   } else {
 #pragma unroll
@@ -310,15 +311,18 @@ template <typename O> struct Kept {
   static __device__ __forceinline__ float value(O hi, int lo) {
     return (float)hi + (float)lo * (__uint_as_float(exponent(hi) < 0x7F000000u ? exponent(hi) : 0u) * (1.f / kUnits));
   }
+  template <bool ONCE>
   __device__ __forceinline__ void put(int which, int64_t at, const float *v, int64_t left, bool wide) const {
-    store_row<O>(p + which * count + at, v, left, wide);
+    store_row<ONCE>(p + which * count + at, v, left, wide);
     if constexpr (kMore) {
       int8_t *to = q + which * count + at;
       if (wide && left >= 8) {
         uint32_t w[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i / 4] |= ((uint32_t)more(v[i]) & 255u) << (i % 4 * 8);
-        *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+        const uint64_t both = (uint64_t)w[0] | (uint64_t)w[1] << 32;
+        if constexpr (ONCE) __builtin_nontemporal_store(both, reinterpret_cast<uint64_t *>(to));
+        else *reinterpret_cast<uint64_t *>(to) = both;
       } else {
         for (int i = 0; i < 8; ++i)
           if (i < left) to[i] = (int8_t)more(v[i]);
@@ -332,17 +336,17 @@ template <typename O> struct Kept {
     if constexpr (!kMore) {
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
-        if (ALIGNED) load_floats<O, 4>(from + i, v + i);
+        if (ALIGNED) load_floats_once<O, 4>(from + i, v + i);
         else
           for (int e = i; e < i + 4; ++e) v[e] = e < left ? (float)from[e] : 0.f;
       }
     } else {
       const int8_t *more = q + which * count + at;
       if constexpr (ALIGNED) {
-        const auto hi = *reinterpret_cast<const typename Pack<O, 8>::type *>(from);
-        const uint2 lo = *reinterpret_cast<const uint2 *>(more);
+        const auto hi = __builtin_nontemporal_load(reinterpret_cast<const typename Pack<O, 8>::type *>(from));
+        const uint64_t lo = __builtin_nontemporal_load(reinterpret_cast<const uint64_t *>(more));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = value(hi[i], (int8_t)((i < 4 ? lo.x : lo.y) >> (i % 4 * 8)));
+        for (int i = 0; i < 8; ++i) v[i] = value(hi[i], (int8_t)(lo >> (i * 8)));
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = i < left ? value(from[i], more[i]) : 0.f;
@@ -439,16 +443,20 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
 
   // A lane holds 4 neighbouring columns of row (lane & 15) in every block of 16 x 16.  Turned in
   // LDS, a lane gets 8 neighbouring columns of a row: stores of 16 bytes.
-  float *turn = reinterpret_cast<float *>(lds) + w * (64 * C::kPitch);
+  // Where a wave's columns of a row fill whole lines of 128 bytes, the results go past the caches,
+  // which keep the operands instead: 1085 -> 1045 us for 16384 x 2048 -> 8192 in bfloat16 with the
+  // projections kept (with half lines it is 1160).
+  constexpr bool kOnce = EPI == kGated && kHalf * sizeof(O) >= 128;
+  float *turn = reinterpret_cast<float *>(lds) + w * (C::kTurnRows * C::kPitch);
   const bool wide = g.wide != 0;
 #pragma unroll
-  for (int h = 0; h < C::kMi / 4; ++h) {
+  for (int h = 0; h < C::kMi / C::kTurnBlocks; ++h) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < C::kTurnBlocks; ++i)
 #pragma unroll
       for (int j = 0; j < C::kNi; ++j)
         *reinterpret_cast<f32x4 *>(turn + (i * 16 + (lane & 15)) * C::kPitch + j * 16 +
-                                   (lane >> 4) * 4) = acc[j][h * 4 + i];
+                                   (lane >> 4) * 4) = acc[j][h * C::kTurnBlocks + i];
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -457,8 +465,8 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
     const int64_t left = g.n - col;
     if (left > 0) {
 #pragma unroll 1
-      for (int r = lane / kAcross; r < 64; r += 64 / kAcross) {
-        const int64_t row = m0 + wm * (C::kMi * 16) + h * 64 + r;
+      for (int r = lane / kAcross; r < C::kTurnRows; r += 64 / kAcross) {
+        const int64_t row = m0 + wm * (C::kMi * 16) + h * C::kTurnRows + r;
         if (row >= g.m) break;
         const float *from = turn + r * C::kPitch + lane % kAcross * 8;
         float a[8];
@@ -472,13 +480,13 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
             for (int e = 0; e < 8 && e < left; ++e) b[e] += (float)static_cast<const O *>(g.bias_b)[col + e];
           if (g.kept != nullptr) {
             const Kept<O> kept(g.kept, g.m, g.n);
-            kept.put(0, row * g.n + col, a, left, wide);
-            kept.put(1, row * g.n + col, b, left, wide);
+            kept.template put<kOnce>(0, row * g.n + col, a, left, wide);
+            kept.template put<kOnce>(1, row * g.n + col, b, left, wide);
           }
           activate<8>(g.act, a, f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[e] *= b[e];
-          store_row<O>(static_cast<O *>(g.out) + row * g.ldo + col, f, left, wide);
+          store_row<kOnce>(static_cast<O *>(g.out) + row * g.ldo + col, f, left, wide);
         } else {
           const bool other = row >= g.second;
           const int64_t r2 = other ? row - g.second : row;
@@ -486,7 +494,7 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
           O *y;  // (a slice's rows: those of out and of out2, one behind the other)
           if (EPI == kPartial) y = static_cast<O *>(g.out) + ((blockIdx.z * (g.second < g.m ? 2 : 1) + (other ? 1 : 0)) * g.each + r2) * g.ldo;
           else y = static_cast<O *>(other ? g.out2 : g.out) + r2 * g.ldo;
-          store_row<O>(y + col, a, left, wide);
+          store_row<false>(y + col, a, left, wide);
         }
       }
     }
