@@ -57,19 +57,27 @@ __device__ __forceinline__ void put_chunk(typename Split<T>::P *to, int64_t stri
   }
 }
 
-// src [rows, cols] -> dst [rows][PARTS][padded]: for rows that are no multiple of 16 bytes, and
-// for floats.
+// src [rows, cols] -> dst [rows][PARTS][padded], of three matrices in one launch: for rows that are
+// no multiple of 16 bytes, and for floats.
+template <typename T> struct PackArgs {
+  const T *src[3];
+  typename Split<T>::P *dst[3];
+  int64_t end[3];  // chunks of 8 columns up to and with this matrix
+  int64_t cols, padded;
+};
 template <typename T>
-__global__ void __launch_bounds__(256)
-    pack_rows_kernel(const T *__restrict__ src, int64_t rows, int64_t cols, int64_t padded,
-                     typename Split<T>::P *__restrict__ dst) {
-  const int64_t chunks = padded / 8, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= rows * chunks) return;
+__global__ void __launch_bounds__(256) pack_rows_kernel(const PackArgs<T> p) {
+  const int64_t chunks = p.padded / 8;
+  int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= p.end[2]) return;
+  const int which = at < p.end[0] ? 0 : at < p.end[1] ? 1 : 2;
+  if (which > 0) at -= p.end[which - 1];
   const int64_t r = at / chunks, c = (at - r * chunks) * 8;
+  const T *src = p.src[which] + r * p.cols + c;
   float v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? (float)src[r * cols + c + i] : 0.f;
-  put_chunk<T>(dst + (r * Split<T>::PARTS) * padded + c, padded, v);
+  for (int i = 0; i < 8; ++i) v[i] = c + i < p.cols ? (float)src[i] : 0.f;
+  put_chunk<T>(p.dst[which] + (r * Split<T>::PARTS) * p.padded + c, p.padded, v);
 }
 
 // da and db, rounded (in parts): g [m][PARTS][2 hp], da at 0 .., db at hp .., zeros behind h; and the
@@ -321,11 +329,12 @@ struct Shape {
   int64_t m, n, k;
 };
 
-// Slices along k of a product with too few tiles to fill the chip (at least 4 steps each).
+// Slices along k of a product with too few tiles to fill the chip; at least 8 steps each, or the
+// launch that adds them up costs more than they save.
 template <typename C> int slices_of(const Shape &s) {
   const int64_t tiles = tiles_of<C>(s.m, s.n), steps = ceil_div(s.k, C::BK);
   int64_t z = tiles >= kCUs ? 1 : 2 * kCUs / tiles;
-  if (z > steps / 4) z = steps / 4;
+  if (z > steps / 8) z = steps / 8;
   if (z < 1) z = 1;
   return (int)ceil_div(steps, ceil_div(steps, z));
 }
@@ -384,15 +393,6 @@ int product(GemmArgs g, float *part, hipStream_t s) {
   return SSC_OK;
 }
 
-template <typename T>
-int pack_rows(const void *src, int64_t rows, int64_t cols, int64_t padded, void *dst, hipStream_t s) {
-  hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((uint32_t)ceil_div(rows * (padded / 8), 256)), dim3(256), 0,
-                     s, static_cast<const T *>(src), rows, cols, padded,
-                     static_cast<typename Split<T>::P *>(dst));
-  SSC_LAUNCH_CHECK("pack_rows_kernel");
-  return SSC_OK;
-}
-
 // Whether the matrix kernel reads the user's rows as they are.
 template <typename T> bool reads_plain(int64_t k, const void *x, const void *wg, const void *wu) {
   return Split<T>::PARTS == 1 && k % 8 == 0 && at16(x) && at16(wg) && at16(wu);
@@ -423,10 +423,20 @@ template <typename T> struct Rows {
       wu.p = wu0;
     } else {
       P *xp = c.take<P>(p.m * kp * PARTS), *gp = c.take<P>(p.h * kp * PARTS), *up = c.take<P>(p.h * kp * PARTS);
-      int rc = pack_rows<T>(x0, p.m, p.k, kp, xp, s);
-      if (rc == SSC_OK) rc = pack_rows<T>(wg0, p.h, p.k, kp, gp, s);
-      if (rc == SSC_OK) rc = pack_rows<T>(wu0, p.h, p.k, kp, up, s);
-      if (rc != SSC_OK) return rc;
+      PackArgs<T> a;
+      a.src[0] = static_cast<const T *>(x0);
+      a.src[1] = static_cast<const T *>(wg0);
+      a.src[2] = static_cast<const T *>(wu0);
+      a.dst[0] = xp;
+      a.dst[1] = gp;
+      a.dst[2] = up;
+      a.end[0] = p.m * (kp / 8);
+      a.end[1] = a.end[0] + p.h * (kp / 8);
+      a.end[2] = a.end[1] + p.h * (kp / 8);
+      a.cols = p.k;
+      a.padded = kp;
+      hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((uint32_t)ceil_div(a.end[2], 256)), dim3(256), 0, s, a);
+      SSC_LAUNCH_CHECK("pack_rows_kernel");
       x.p = xp;
       wg.p = gp;
       wu.p = up;

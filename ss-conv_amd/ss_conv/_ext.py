@@ -1872,28 +1872,35 @@ ELEM = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACT_SILU, ACT_GELU = 4, 5
 
 
-def on_device_of(t):
-    """A context in which native launches go to the device of `t`."""
-    return torch.cuda.device(t.device)
+def call_on(t, fn, *args):
+    """fn(*args) with the device of `t` as the current one, which native launches go to."""
+    if t.get_device() == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(t.device):
+        return fn(*args)
+
+
+# (the number of a device's current stream without a Stream object around it)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def groupnorm_forward(x, offsets, groups, weight, bias, eps, act):
-    """y[n, c], mean[clouds, groups], rstd[clouds, groups] of contiguous rows x[n, c]."""
+    """y[n, c] and stats[2, clouds, groups] (mean, 1 / sqrt(var + eps)) of contiguous rows x[n, c]."""
     n, c = x.shape
     clouds = offsets.numel() - 1
     y = torch.empty_like(x)
     stats = torch.empty((2, clouds, groups), dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind()
     ws = _workspace(_lib.ssc_groupnorm_workspace_bytes(n, c, clouds, groups), x.device)
-    wtype = ELEM[(x if weight is None else weight).dtype] if bias is None else ELEM[bias.dtype]
+    mean = stats.data_ptr()
     _check(_lib.ssc_groupnorm_fwd(
-        ELEM[x.dtype], _ptr(x), n, c, offsets.data_ptr(), clouds, groups, wtype, _ptr(weight),
-        _ptr(bias), eps, act, _ptr(y), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), ws.numel(),
-        _stream(x)))
-    return y, mean, rstd
+        ELEM[x.dtype], _ptr(x), n, c, offsets.data_ptr(), clouds, groups,
+        _param_elem(x, weight, bias), _ptr(weight), _ptr(bias), eps, act, _ptr(y), mean,
+        mean + 4 * clouds * groups, ws.data_ptr(), ws.numel(), _raw_stream(x.get_device())))
+    return y, stats
 
 
-def groupnorm_backward(x, dy, offsets, groups, weight, bias, act, mean, rstd, want):
+def groupnorm_backward(x, dy, offsets, groups, weight, bias, act, stats, want):
     """dx, dweight, dbias (None where `want` says so) of contiguous rows x, dy [n, c], n >= 1."""
     n, c = x.shape
     clouds = offsets.numel() - 1
@@ -1901,12 +1908,18 @@ def groupnorm_backward(x, dy, offsets, groups, weight, bias, act, mean, rstd, wa
     dweight = torch.empty_like(weight) if want[1] else None
     dbias = torch.empty_like(bias) if want[2] else None
     ws = _workspace(_lib.ssc_groupnorm_workspace_bytes(n, c, clouds, groups), x.device)
-    wtype = ELEM[(x if weight is None else weight).dtype] if bias is None else ELEM[bias.dtype]
+    mean = stats.data_ptr()
     _check(_lib.ssc_groupnorm_bwd(
-        ELEM[x.dtype], x.data_ptr(), dy.data_ptr(), n, c, offsets.data_ptr(), clouds, groups, wtype,
-        _ptr(weight), _ptr(bias), act, mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dweight),
-        _ptr(dbias), ws.data_ptr(), ws.numel(), _stream(x)))
+        ELEM[x.dtype], x.data_ptr(), dy.data_ptr(), n, c, offsets.data_ptr(), clouds, groups,
+        _param_elem(x, weight, bias), _ptr(weight), _ptr(bias), act, mean,
+        mean + 4 * clouds * groups, _ptr(dx), _ptr(dweight), _ptr(dbias), ws.data_ptr(),
+        ws.numel(), _raw_stream(x.get_device())))
     return dx, dweight, dbias
+
+
+def _param_elem(x, weight, bias):
+    """Element type of the parameters: both have the same, where there are any."""
+    return ELEM[(weight if weight is not None else bias if bias is not None else x).dtype]
 
 
 def gated_forward(x, w_gate, w_up, b_gate, b_up, act, keep):
@@ -1920,7 +1933,7 @@ def gated_forward(x, w_gate, w_up, b_gate, b_up, act, keep):
     ws = _workspace(_lib.ssc_gated_fwd_workspace_bytes(elem, m, k, h), x.device)
     _check(_lib.ssc_gated_fwd(elem, _ptr(x), m, k, w_gate.data_ptr(), w_up.data_ptr(), h,
                               _ptr(b_gate), _ptr(b_up), act, _ptr(y), _ptr(kept), ws.data_ptr(),
-                              ws.numel(), _stream(x)))
+                              ws.numel(), _raw_stream(x.get_device())))
     return y, kept
 
 
@@ -1938,7 +1951,7 @@ def gated_backward(x, w_gate, w_up, act, kept, dy, want):
     _check(_lib.ssc_gated_bwd(elem, x.data_ptr(), m, k, w_gate.data_ptr(), w_up.data_ptr(), h, act,
                               kept.data_ptr(), dy.data_ptr(), _ptr(dx), _ptr(dw_gate),
                               _ptr(dw_up), _ptr(db_gate), _ptr(db_up), ws.data_ptr(), ws.numel(),
-                              _stream(x)))
+                              _raw_stream(x.get_device())))
     return dx, dw_gate if want[1] else None, dw_up if want[2] else None, db_gate, db_up
 
 

@@ -36,9 +36,8 @@ class _GatedLinear(torch.autograd.Function):
         if x.size(0) == 0:
             shapes = (x, w_gate, w_up, w_gate[:, 0], w_gate[:, 0])
             return tuple(torch.zeros_like(t) if w else None for t, w in zip(shapes, want)) + (None,)
-        with _ext.on_device_of(x):
-            return _ext.gated_backward(x, w_gate, w_up, ctx.act, kept, dy.contiguous(), want) + \
-                (None,)
+        return _ext.call_on(x, _ext.gated_backward, x, w_gate, w_up, ctx.act, kept,
+                            dy.contiguous(), want) + (None,)
 
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
@@ -62,15 +61,14 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
         pointwise.check_like(what, t, shape, (x.dtype,), x.device)
     if w_up is None:
         raise TypeError("w_up is missing")
-    rows = x.reshape(-1, k).contiguous()
+    rows = (x if x.dim() == 2 else x.reshape(-1, k)).contiguous()
     w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
     b_gate, b_up = [None if t is None else t.contiguous() for t in (b_gate, b_up)]
-    with _ext.on_device_of(x):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                           for t in (rows, w_gate, w_up, b_gate, b_up)):
-            y = _GatedLinear.apply(rows, w_gate, w_up, b_gate, b_up, act)
-        else:
-            y = _ext.gated_forward(rows, w_gate, w_up, b_gate, b_up, act, False)[0]
+    args = (rows, w_gate, w_up, b_gate, b_up)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        y = _ext.call_on(x, _GatedLinear.apply, *args, act)
+    else:
+        y = _ext.call_on(x, _ext.gated_forward, *args, act, False)[0]
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (h,))
 
 

@@ -21,23 +21,21 @@ from ss_conv import pointwise
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, offsets, groups, eps, act):
-        y, mean, rstd = _ext.groupnorm_forward(x, offsets, groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, offsets, mean, rstd)
+        y, stats = _ext.groupnorm_forward(x, offsets, groups, weight, bias, eps, act)
+        ctx.save_for_backward(x, weight, bias, offsets, stats)
         ctx.groups, ctx.act = groups, act
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, offsets, mean, rstd = ctx.saved_tensors
+        x, weight, bias, offsets, stats = ctx.saved_tensors
         want = ctx.needs_input_grad[:3]
         if x.size(0) == 0:
             made = [torch.zeros_like(t) if w else None for t, w in zip((x, weight, bias), want)]
             return tuple(made) + (None,) * 4
-        with _ext.on_device_of(x):
-            grads = _ext.groupnorm_backward(x, dy.contiguous(), offsets, ctx.groups, weight, bias,
-                                            ctx.act, mean, rstd, want)
-        return grads + (None,) * 4
+        return _ext.call_on(x, _ext.groupnorm_backward, x, dy.contiguous(), offsets, ctx.groups,
+                            weight, bias, ctx.act, stats, want) + (None,) * 4
 
 
 def group_norm(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
@@ -72,14 +70,15 @@ def group_norm(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activat
         raise TypeError("weight has type {}, bias {}".format(weight.dtype, bias.dtype))
     offsets = offsets.to(torch.int32).contiguous()
     x = x.contiguous()
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    with _ext.on_device_of(x):
-        if torch.is_grad_enabled() and (
-                x.requires_grad or (weight is not None and weight.requires_grad) or
-                (bias is not None and bias.requires_grad)):
-            return _GroupNorm.apply(x, weight, bias, offsets, num_groups, eps, act)
-        return _ext.groupnorm_forward(x, offsets, num_groups, weight, bias, eps, act)[0]
+    grad = x.requires_grad
+    if weight is not None:
+        weight, grad = weight.contiguous(), grad or weight.requires_grad
+    if bias is not None:
+        bias, grad = bias.contiguous(), grad or bias.requires_grad
+    if grad and torch.is_grad_enabled():
+        return _ext.call_on(x, _GroupNorm.apply, x, weight, bias, offsets, num_groups, eps, act)
+    return _ext.call_on(x, _ext.groupnorm_forward, x, offsets, num_groups, weight, bias, eps,
+                        act)[0]
 
 
 class GroupNorm(nn.Module):

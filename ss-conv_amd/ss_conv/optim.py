@@ -78,28 +78,28 @@ def _check_order(i, p, items):
                                             p.stride()))
 
 
-_dtype, _shape, _layout = [operator.attrgetter(n) for n in ("dtype", "shape", "layout")]
+_dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
 
 
-def _usual(params, lists, dtypes):
-    """Whether all tensors are contiguous, on one GPU and as the checks want them: one pass over
-    each list for each property, where the checks tensor by tensor take several times as long."""
-    shapes = list(map(_shape, params))
-    kinds = list(map(_dtype, params))
-    several = [params] + lists
-    return (all(set(map(_layout, x)) == {torch.strided} for x in several) and
-            all(map(torch.Tensor.is_contiguous, itertools.chain(*several))) and
-            len(set(map(torch.Tensor.get_device, itertools.chain(*several)))) == 1 and
-            params[0].is_cuda and set(kinds) <= _ext.ELEM.keys() and
-            list(map(_dtype, lists[0])) == kinds and
-            all(list(map(_shape, x)) == shapes for x in lists[:3]) and
-            all(set(map(_dtype, x)) == {t} for x, t in zip(lists[1:], dtypes)) and
-            all(list(map(torch.Tensor.numel, x)) == [_scales(p.numel()) for p in params]
-                for x in lists[3:]))
+def _usual(first, others, dtypes, sizes, blocks):
+    """Whether all tensors are contiguous and on one GPU, the i-th list of `others` is of dtypes[i]
+    and its tensors have `sizes` elements, or one for each block where blocks[i]: one pass over
+    the lists for each property, where checks tensor by tensor take several times as long."""
+    every = list(itertools.chain(first, *others))
+    try:
+        alike = all(map(torch.Tensor.is_contiguous, every))
+    except RuntimeError:  # (sparse tensors do not say)
+        return False
+    if not alike or not first[0].is_cuda or len(set(map(torch.Tensor.get_device, every))) != 1:
+        return False
+    scales = [_scales(n) for n in sizes] if any(blocks[:len(others)]) else None
+    return all(set(map(_dtype, x)) == {t} and list(map(torch.Tensor.numel, x)) ==
+               (scales if b else sizes) for x, t, b in zip(others, dtypes, blocks))
 
 
 _BITS8 = (torch.int8, torch.uint8, torch.float32, torch.float32)
 _BITS32 = (torch.float32, torch.float32)
+_BLOCKS = (False, False, True, True)  # which of them have one element for each block
 
 
 def _scales(n):
@@ -126,7 +126,10 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.99
         return
     dtypes = _BITS8 if eight else _BITS32
     dev = params[0].device
-    if not _usual(params, lists, dtypes):
+    sizes, kinds = list(map(torch.Tensor.numel, params)), list(map(_dtype, params))
+    if not (set(kinds) <= _ext.ELEM.keys() and list(map(_dtype, grads)) == kinds and
+            list(map(_shape, grads)) == list(map(_shape, params)) and
+            _usual(list(params) + list(grads), lists[1:], dtypes, sizes, _BLOCKS)):
         lists[0] = grads = list(grads)
         for i, p in enumerate(params):
             _check_param(i, p, grads[i])
@@ -141,19 +144,18 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.99
     columns = [map(torch.Tensor.data_ptr, x) for x in [params] + lists]
     if not eight:
         columns += [itertools.repeat(0)] * 2
-    columns += [map(torch.Tensor.numel, params), [_ext.ELEM[p.dtype] for p in params]]
-    with torch.cuda.device(dev):
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("an AdamW step cannot be captured into a graph: the number of the "
-                               "step is an argument of its launch")
-        _ext.adamw_step(columns, count, 8 if eight else 32, lr, betas[0], betas[1], eps,
-                        weight_decay, step, torch.cuda.current_stream(dev).cuda_stream)
+    columns += [sizes, [_ext.ELEM[t] for t in kinds]]
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("an AdamW step cannot be captured into a graph: the number of the step "
+                           "is an argument of its launch")
+    _ext.call_on(params[0], _ext.adamw_step, columns, count, 8 if eight else 32, lr, betas[0],
+                 betas[1], eps, weight_decay, step, _ext._raw_stream(dev.index))
     torch.autograd.graph.increment_version(params)
 
 
 def state_values(exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, out=None):
     """The float32 moments that lists of 8-bit ones stand for: (exp_avgs, exp_avg_sqs).
-    out: the two lists of contiguous float32 tensors to write them to."""
+    out: the two lists of float32 tensors, laid out as the moments, to write them to."""
     count = len(exp_avgs)
     lists = [exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales] + (list(out) if out is not None else [])
     if any(len(x) != count for x in lists):
@@ -164,21 +166,20 @@ def state_values(exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, out=N
     dev = exp_avgs[0].device
     _ext._need_gpu(exp_avgs[0])
     if out is None:
-        out = tuple([torch.empty(t.shape, dtype=torch.float32, device=dev) for t in x]
+        out = tuple([torch.empty_like(t, dtype=torch.float32) for t in x]
                     for x in (exp_avgs, exp_avg_sqs))
     moments = [exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales]
-    for i, m in enumerate(exp_avgs):
-        n = m.numel()
-        _check_moments(i, n, dev, [x[i] for x in moments], _BITS8, (n, n, _scales(n), _scales(n)))
-        for t in (out[0][i], out[1][i]):
-            if t.dtype is not torch.float32 or t.numel() != n or t.device != dev or \
-                    not t.is_contiguous():
-                raise ValueError("out of tensor {}: {} contiguous float32 elements are "
-                                 "needed".format(i, n))
+    sizes = list(map(torch.Tensor.numel, exp_avgs))
+    if not _usual(exp_avgs, moments + list(out), _BITS8 + _BITS32, sizes, _BLOCKS + _BLOCKS[:2]):
+        for i, n in enumerate(sizes):
+            _check_moments(i, n, dev, [x[i] for x in moments], _BITS8,
+                           (n, n, _scales(n), _scales(n)))
+            _check_moments(i, n, dev, (out[0][i], out[1][i]), _BITS32, (n, n))
+            # (a new tensor has the layout of the codes, a given one has to have it)
+            _check_order(i, exp_avgs[i], (exp_avg_sqs[i], out[0][i], out[1][i]))
     columns = [map(torch.Tensor.data_ptr, x) for x in list(out) + moments]
-    columns += [map(torch.Tensor.numel, exp_avgs), itertools.repeat(0)]
-    with torch.cuda.device(dev):
-        _ext.adamw_values(columns, count, torch.cuda.current_stream(dev).cuda_stream)
+    columns += [sizes, itertools.repeat(0)]
+    _ext.call_on(exp_avgs[0], _ext.adamw_values, columns, count, _ext._raw_stream(dev.index))
     return tuple(out)
 
 

@@ -50,7 +50,8 @@ def check_rows(what, x):
 
 def check_like(what, t, shape, dtypes, device):
     """An optional tensor of a given shape, type and device."""
-    if t is None:
+    if t is None or (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype in dtypes and
+                     t.device == device):
         return
     if not torch.is_tensor(t):
         raise TypeError("{} is a {}, not a tensor".format(what, type(t).__name__))
