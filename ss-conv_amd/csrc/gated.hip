@@ -6,8 +6,8 @@
 //
 // Forward: one launch of the matrix kernel (gated_gemm.h) whose tiles hold the same columns of
 // both projections, so activation and product happen in registers and neither projection goes
-// through memory (a training step keeps a and b, in 24 or 32 bits, for the backward pass); up to
-// kFewRows rows a kernel that streams the weights once.  Backward: one pass makes da and db, side
+// through memory (a training step keeps a and b, in 24 or 32 bits, for the backward pass); for few
+// rows a kernel that streams the weights from memory into the matrix instructions.  Backward: one pass makes da and db, side
 // by side, then one product gives dx (k runs over both projections' columns) and one gives both
 // weight gradients (k runs over the rows, cut into slices where there are few tiles; slices are
 // added in order).
@@ -16,8 +16,6 @@
 
 namespace ssc {
 namespace {
-
-constexpr int kFewRows = 32;
 
 // ---- operands of the matrix kernel ----------------------------------------------------------
 // How an element of the user's arrays becomes PARTS 16-bit ones.
@@ -81,24 +79,29 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const PackArgs<T> p) {
 }
 
 // da and db, rounded (in parts): g [m][PARTS][2 hp], da at 0 .., db at hp .., zeros behind h; and the
-// column sums of every kGradRows rows, sums [tiles of rows][2 h] (NULL: not wanted).  8
+// column sums of every `rows` rows, sums [tiles of rows][2 h] (NULL: not wanted).  8
 // neighbouring columns of a row to a thread; ALIGNED: rows begin at 16 bytes.  HBM-bound.
-constexpr int kGradRows = 64, kGradAcross = 32;  // rows of a workgroup, threads side by side
+constexpr int kGradAcross = 32;  // threads side by side
+// Rows of a workgroup: 64, or 16 where that leaves too few workgroups.
+int grad_rows(int64_t m, int64_t hp) {
+  return ceil_div(m, 64) * ceil_div(hp, kGradAcross * 8) >= 512 ? 64 : 16;
+}
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256)
     gated_grad_kernel(const T *__restrict__ dy, const void *__restrict__ ab, int64_t m, int64_t h, int act,
-                      int64_t hp, typename Split<T>::P *__restrict__ g, float *__restrict__ sums) {
+                      int64_t hp, int rows, typename Split<T>::P *__restrict__ g,
+                      float *__restrict__ sums) {
   const Kept<T> kept(ab, m, h);
   constexpr int kDown = 256 / kGradAcross;
   __shared__ float lds[kDown][kGradAcross * 8 + 1];
   const int cx = threadIdx.x % kGradAcross, row = threadIdx.x / kGradAcross;
-  const int64_t c = ((int64_t)blockIdx.y * kGradAcross + cx) * 8, r0 = (int64_t)blockIdx.x * kGradRows;
+  const int64_t c = ((int64_t)blockIdx.y * kGradAcross + cx) * 8, r0 = (int64_t)blockIdx.x * rows;
   float sa[8], sb[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sa[i] = sb[i] = 0.f;
   if (c < hp) {
 #pragma unroll 2
-    for (int64_t r = r0 + row; r < r0 + kGradRows; r += kDown) {
+    for (int64_t r = r0 + row; r < r0 + rows; r += kDown) {
       if (r >= m) break;
       float yv[8], av[8], bv[8], f[8], d[8];
       const int64_t at = r * h + c;
@@ -181,12 +184,13 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- few rows -------------------------------------------------------------------------------
-// 16 hidden columns of both projections, up to 16 MT rows; the waves of the workgroup take the
-// steps along k in turn and are added up in LDS.  Bound by the weights' bytes: a lane reads 32
-// neighbouring bytes of a row of the weights at a step, and rows (16 lanes) and steps are
-// independent, so many loads are in flight.  k is dealt to the lanes as the weights lie in
-// memory, not in the matrix instruction's own order: a sum does not mind as long as x is dealt
-// alike.
+// 16 hidden columns of both projections, 16 MT rows; the waves of the workgroup take the steps along
+// k in turn and are added up in LDS.  Bound by the weights' bytes up to some 32 rows (one row through
+// 4096 -> 8192 in bfloat16: 27 us, 5.0 TB/s; 32 rows 34 us), by the matrix units' waiting for them
+// beyond: a lane reads 32 neighbouring bytes of a row of the weights at a step, and rows (16 lanes)
+// and steps are independent, so many loads are in flight.  k is dealt to the lanes as the weights
+// lie in memory, not in the matrix instruction's own order: a sum does not mind as long as x is
+// dealt alike.  Float elements go to float matrix instructions as they are.
 template <typename T> struct FewStep;  // one step: 64 elements along k (16 bits), 32 (float)
 template <> struct FewStep<f16> { static constexpr int kLane = 16; };
 template <> struct FewStep<bf16> { static constexpr int kLane = 16; };
@@ -235,12 +239,12 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmArgs g) {
   __shared__ f32x4 lds[W][2 * MT][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int64_t col = n0 + r < g.n ? n0 + r : g.n - 1;
+  const int64_t col = n0 + r < g.n ? n0 + r : g.n - 1, m0 = (int64_t)blockIdx.y * 16 * MT;
   const T *wg = static_cast<const T *>(g.b.p) + col * g.b.ld, *wu = static_cast<const T *>(g.b.q) + col * g.b.ld;
   const T *x[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
-    x[t] = static_cast<const T *>(g.a.p) + (t * 16 + r < g.m ? t * 16 + r : g.m - 1) * g.a.ld;
+    x[t] = static_cast<const T *>(g.a.p) + (m0 + t * 16 + r < g.m ? m0 + t * 16 + r : g.m - 1) * g.a.ld;
   f32x4 acc[2 * MT];
 #pragma unroll
   for (int t = 0; t < 2 * MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -281,7 +285,7 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmArgs g) {
     sa += lds[v][2 * w][lane];
     sb += lds[v][2 * w + 1][lane];
   }
-  const int64_t row = w * 16 + r, c0 = n0 + q * 4;
+  const int64_t row = m0 + w * 16 + r, c0 = n0 + q * 4;
   if (row >= g.m) return;
   float a[4], b[4], f[4];
 #pragma unroll
@@ -308,7 +312,8 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmArgs g) {
 int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 bool at16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Tiles: large ones reuse more of what they read, small ones fill the chip where there are few.
+// Tiles: large ones reuse more of what they read, small ones fill the chip where there are few, and
+// several of them share a CU, so that one's results are stored while another one multiplies.
 template <typename T> struct Tiles {
   typedef Tile<T, 1, 256, 256, 64, 4, 2> Large;
   typedef Tile<T, 1, 128, 128, 64, 2, 2> Middle;
@@ -316,8 +321,7 @@ template <typename T> struct Tiles {
 };
 template <> struct Tiles<float> {
   typedef Tile<bf16, 3, 256, 128, 32, 4, 2> Large;
-  typedef Tile<bf16, 3, 128, 128, 32, 2, 2> Middle;
-  typedef Tile<bf16, 3, 64, 128, 32, 1, 4> Small;
+  typedef Tile<bf16, 3, 64, 128, 32, 1, 4> Middle, Small;
 };
 constexpr int kCUs = 256;
 
@@ -338,19 +342,28 @@ template <typename C> int slices_of(const Shape &s) {
   if (z < 1) z = 1;
   return (int)ceil_div(steps, ceil_div(steps, z));
 }
-// 2: large tiles, 1: middle ones, 0: small ones
-template <typename T> int size_of(const Shape &s, bool sliced) {
-  if (sliced) {
-    // (work per tile counts: a sliced product fills the chip with any of them)
-    if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) * s.k >= (int64_t)kCUs * 2048) return 2;
-    return s.m > 64 ? 1 : 0;
-  }
-  if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) >= kCUs) return 2;
-  if (tiles_of<typename Tiles<T>::Middle>(s.m, s.n) >= kCUs) return 1;
-  return 0;
+// 2: large tiles, 1: middle ones, 0: small ones (float: large or small).
+//
+// Forward: large tiles where they fill the chip, unless both projections are kept and k is short:
+// storing takes longer than multiplying then, and a CU holds only one large tile.  25600 rows ->
+// 1024, kept, bfloat16, large against middle tiles: k = 128 73 and 66 us, 256 82 and 81, 512 105 and
+// 110; floats, large against small: k = 128 195 and 148 us, 256 256 and 243, 512 387 and 403.
+template <typename T> int forward_size(const Shape &s, bool kept) {
+  if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) >= kCUs && !(kept && s.k <= 384)) return 2;
+  return tiles_of<typename Tiles<T>::Middle>(s.m, s.n) >= kCUs ? 1 : 0;
+}
+// The products of the backward pass are sliced where tiles are few, so they fill the chip with any
+// of them; the tile's reuse counts for more the longer the product takes (times with the pass that
+// makes da and db).  bfloat16, large, middle, small: 25600 x 2048 (k) x 2048 293, 363, 377 us; 25600 x
+// 1024 (k) x 2048 207, 203, 283; 16384 x 512 (k) x 2048 101, 74, 78; 1024 x 2048 (k) x 2048 49, 45, 38.
+template <typename T> int product_size(const Shape &s) {
+  const double work = (double)s.m * s.n * s.k;
+  if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) >= kCUs * 3 / 4) return 2;
+  if (work >= (sizeof(T) == 4 ? 2e10 : 8e10)) return 2;
+  return tiles_of<typename Tiles<T>::Middle>(s.m, s.n) >= kCUs || work >= 1.2e10 ? 1 : 0;
 }
 template <typename T> int slices_for(const Shape &s) {
-  const int z = size_of<T>(s, true);
+  const int z = product_size<T>(s);
   return z == 2 ? slices_of<typename Tiles<T>::Large>(s)
                 : z == 1 ? slices_of<typename Tiles<T>::Middle>(s) : slices_of<typename Tiles<T>::Small>(s);
 }
@@ -371,7 +384,7 @@ int launch(GemmArgs g, int64_t n_tile, int slices, hipStream_t s) {
 template <typename T, bool TA, bool TB>
 int product(GemmArgs g, float *part, hipStream_t s) {
   const Shape shape = {g.m, g.n, g.k};
-  const int size = size_of<T>(shape, true), slices = slices_for<T>(shape);
+  const int size = product_size<T>(shape), slices = slices_for<T>(shape);
   typedef Tiles<T> S;
   if (slices == 1) {
     g.wide = (g.ldo * sizeof(T)) % 16 == 0 && at16(g.out) && at16(g.out2);
@@ -401,6 +414,16 @@ template <typename T> bool reads_plain(int64_t k, const void *x, const void *wg,
 struct Problem {
   int64_t m, k, h;
 };
+
+// Whether the few-rows kernel is taken: for 16 bits up to 64 rows, or a workgroup to a CU; for
+// floats, which it takes as they are where tiles want them in parts, up to 896 workgroups.  It
+// against tiles, us: bfloat16, 1024 -> 1024, 256 rows 9.5 and 10.5, 384 rows 14.8 and 10.7; 2048 ->
+// 4096, 64 rows 16 and 22, 96 rows 24 and 22; floats, 1000 -> 2728, 256 rows 47 and 57, 512 rows 89
+// and 84; 2048 -> 4096, 192 rows 90 and 107, 256 rows 122 and 113; 128 -> 512, 512 rows 5.6 and 11.
+template <typename T> bool takes_few(const Problem &p) {
+  const int64_t groups = ceil_div(p.h, 16) * ceil_div(p.m, 64);
+  return sizeof(T) == 4 ? groups <= 896 : p.m <= 64 || groups <= kCUs;
+}
 
 size_t packed_bytes(int64_t rows, int64_t padded, int parts) {
   return align_up((size_t)rows * padded * parts * 2);
@@ -449,13 +472,14 @@ template <typename T> struct Rows {
 };
 
 template <typename T> size_t forward_bytes(const Problem &p) {
-  return p.m <= kFewRows ? 256 : Rows<T>::bytes(p);
+  return takes_few<T>(p) ? 256 : Rows<T>::bytes(p);
 }
 
 template <typename T, bool ALIGNED> void few_rows(const GemmArgs &g, hipStream_t s) {
-  const dim3 grid((uint32_t)ceil_div(g.n, 16));
+  const dim3 grid((uint32_t)ceil_div(g.n, 16), (uint32_t)ceil_div(g.m, 64));
   if (g.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, ALIGNED>), grid, dim3(512), 0, s, g);
-  else hipLaunchKernelGGL((few_rows_kernel<T, 2, ALIGNED>), grid, dim3(512), 0, s, g);
+  else if (g.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, ALIGNED>), grid, dim3(512), 0, s, g);
+  else hipLaunchKernelGGL((few_rows_kernel<T, 4, ALIGNED>), grid, dim3(512), 0, s, g);
 }
 
 template <typename T>
@@ -470,7 +494,7 @@ int forward(const Problem &p, const void *x, const void *wg, const void *wu, con
   g.out = y;
   g.kept = kept;
   g.ldo = p.h;
-  if (p.m <= kFewRows) {
+  if (takes_few<T>(p)) {
     g.a.p = x;
     g.b.p = wg;
     g.b.q = wu;
@@ -493,7 +517,7 @@ int forward(const Problem &p, const void *x, const void *wg, const void *wu, con
   g.b.q = rows.wu.p;
   g.b.rows = p.h;
   g.wide = (p.h * sizeof(T)) % 16 == 0 && at16(y);
-  const int size = size_of<T>({p.m, 2 * p.h, g.k}, false);
+  const int size = forward_size<T>({p.m, 2 * p.h, g.k}, kept != nullptr);
   typedef Tiles<T> S;
   return size == 2 ? launch<typename S::Large, false, false, kGated, T>(g, 2 * p.h, 1, s)
                    : size == 1 ? launch<typename S::Middle, false, false, kGated, T>(g, 2 * p.h, 1, s)
@@ -504,6 +528,7 @@ template <typename T> struct Backward {
   typedef typename Split<T>::P P;
   static constexpr int PARTS = Split<T>::PARTS;
   int64_t hp;  // columns of da and of db in g: a multiple of every tile's k
+  int rows;    // of a workgroup of the pass that makes g
   P *g;
   float *sums, *part;
   size_t used;
@@ -511,7 +536,8 @@ template <typename T> struct Backward {
     hp = ceil_div(p.h, 64) * 64;
     Carver c(ws);
     g = c.take<P>(p.m * PARTS * 2 * hp);
-    sums = c.take<float>(ceil_div(p.m, kGradRows) * 2 * p.h);
+    rows = grad_rows(p.m, hp);
+    sums = c.take<float>(ceil_div(p.m, rows) * 2 * p.h);
     // the slices of the two products, one after the other
     const int zx = slices_for<T>(dx_shape(p)), zw = slices_for<T>(dw_shape(p));
     const int64_t px = zx > 1 ? zx * p.m * p.k : 0, pw = zw > 1 ? zw * 2 * p.h * p.k : 0;
@@ -530,11 +556,11 @@ int backward(const Problem &p, const void *x, const void *wg, const void *wu, in
   constexpr int PARTS = Split<T>::PARTS;
   const Backward<T> w(p, ws);
   const bool biases = dbg != nullptr || dbu != nullptr;
-  const dim3 tiles((uint32_t)ceil_div(p.m, kGradRows), (uint32_t)ceil_div(w.hp, kGradAcross * 8));
+  const dim3 tiles((uint32_t)ceil_div(p.m, w.rows), (uint32_t)ceil_div(w.hp, kGradAcross * 8));
   const bool aligned = (p.h % 8) == 0 && at16(dy);
 #define SSC_GRAD(ALIGNED)                                                                              \
   hipLaunchKernelGGL((gated_grad_kernel<T, ALIGNED>), tiles, dim3(256), 0, s, static_cast<const T *>(dy), \
-                     kept, p.m, p.h, act, w.hp, w.g,   \
+                     kept, p.m, p.h, act, w.hp, w.rows, w.g, \
                      biases ? w.sums : nullptr)
   if (aligned) SSC_GRAD(true);
   else SSC_GRAD(false);
@@ -542,7 +568,7 @@ int backward(const Problem &p, const void *x, const void *wg, const void *wu, in
   SSC_LAUNCH_CHECK("gated_grad_kernel");
   if (biases) {
     hipLaunchKernelGGL(bias_grad_kernel<T>, dim3((uint32_t)ceil_div(2 * p.h, 16)), dim3(256), 0, s, w.sums,
-                       ceil_div(p.m, kGradRows), p.h, static_cast<T *>(dbg), static_cast<T *>(dbu));
+                       ceil_div(p.m, w.rows), p.h, static_cast<T *>(dbg), static_cast<T *>(dbu));
     SSC_LAUNCH_CHECK("bias_grad_kernel");
   }
   if (dx == nullptr && dwg == nullptr) return SSC_OK;

@@ -448,6 +448,18 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
   // projections kept (with half lines it is 1160).
   constexpr bool kOnce = EPI == kGated && kHalf * sizeof(O) >= 128;
   float *turn = reinterpret_cast<float *>(lds) + w * (C::kTurnRows * C::kPitch);
+  constexpr int kAcross = (EPI == kGated ? kHalf : C::kNi * 16) / 8;  // lanes of a row
+  const int64_t col = n0 + wn * (kAcross * 8) + lane % kAcross * 8;
+  const int64_t left = g.n - col;
+  float bias_a[8], bias_b[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    bias_a[e] = bias_b[e] = 0.f;
+    if (EPI == kGated && e < left) {
+      if (g.bias_a != nullptr) bias_a[e] = (float)static_cast<const O *>(g.bias_a)[col + e];
+      if (g.bias_b != nullptr) bias_b[e] = (float)static_cast<const O *>(g.bias_b)[col + e];
+    }
+  }
   const bool wide = g.wide != 0;
 #pragma unroll
   for (int h = 0; h < C::kMi / C::kTurnBlocks; ++h) {
@@ -460,9 +472,6 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    constexpr int kAcross = (EPI == kGated ? kHalf : C::kNi * 16) / 8;  // lanes of a row
-    const int64_t col = n0 + wn * (kAcross * 8) + lane % kAcross * 8;
-    const int64_t left = g.n - col;
     if (left > 0) {
 #pragma unroll 1
       for (int r = lane / kAcross; r < C::kTurnRows; r += 64 / kAcross) {
@@ -474,10 +483,11 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
         if constexpr (EPI == kGated) {
           float b[8], f[8];
           load_turned(from + kHalf, b);
-          if (g.bias_a != nullptr)
-            for (int e = 0; e < 8 && e < left; ++e) a[e] += (float)static_cast<const O *>(g.bias_a)[col + e];
-          if (g.bias_b != nullptr)
-            for (int e = 0; e < 8 && e < left; ++e) b[e] += (float)static_cast<const O *>(g.bias_b)[col + e];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            a[e] += bias_a[e];
+            b[e] += bias_b[e];
+          }
           if (g.kept != nullptr) {
             const Kept<O> kept(g.kept, g.m, g.n);
             kept.template put<kOnce>(0, row * g.n + col, a, left, wide);
