@@ -18,48 +18,18 @@ namespace ssc {
 namespace {
 
 // ---- operands of the matrix kernel ----------------------------------------------------------
-// How an element of the user's arrays becomes PARTS 16-bit ones.
-template <typename T> struct Split {
-  typedef T P;
-  static constexpr int PARTS = 1;
-  static __device__ __forceinline__ void of(float v, P *p) { p[0] = (T)v; }
-};
-template <> struct Split<float> {
-  typedef bf16 P;
-  static constexpr int PARTS = 3;
-  static __device__ __forceinline__ void of(float v, P *p) {
-    p[0] = (bf16)v;
-    // the largest floats would round to infinity: cut instead
-    if (__builtin_isfinite(v) && !__builtin_isfinite((float)p[0]))
-      p[0] = (bf16)__uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
-    const float r = v - (float)p[0];
-    const bool fine = __builtin_isfinite(r);  // (of an infinity or NaN nothing is left)
-    p[1] = fine ? (bf16)r : (bf16)0.f;
-    p[2] = fine ? (bf16)(r - (float)p[1]) : (bf16)0.f;
-  }
-};
-
-// 8 values as a chunk of each part; parts lie `stride` elements apart.
-template <typename T>
-__device__ __forceinline__ void put_chunk(typename Split<T>::P *to, int64_t stride, const float *v) {
-  typedef typename Split<T>::P P;
-  P parts[8][Split<T>::PARTS];
+// 8 neighbouring elements of an array of the kernels' own.
+template <typename T> __device__ __forceinline__ void put_eight(T *to, const float *v) {
+  constexpr int V = 16 / sizeof(T);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) Split<T>::of(v[i], parts[i]);
-#pragma unroll
-  for (int p = 0; p < Split<T>::PARTS; ++p) {
-    typename Pack<P, 8>::type c;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = parts[i][p];
-    *reinterpret_cast<typename Pack<P, 8>::type *>(to + p * stride) = c;
-  }
+  for (int i = 0; i < 8; i += V) store_floats<T, V>(to + i, v + i);
 }
 
-// src [rows, cols] -> dst [rows][PARTS][padded], of three matrices in one launch: for rows that are
-// no multiple of 16 bytes, and for floats.
+// src [rows, cols] -> dst [rows][padded], of three matrices in one launch: for rows of 16-bit elements
+// that are no multiple of 16 bytes.
 template <typename T> struct PackArgs {
   const T *src[3];
-  typename Split<T>::P *dst[3];
+  T *dst[3];
   int64_t end[3];  // chunks of 8 columns up to and with this matrix
   int64_t cols, padded;
 };
@@ -75,10 +45,10 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const PackArgs<T> p) {
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = c + i < p.cols ? (float)src[i] : 0.f;
-  put_chunk<T>(p.dst[which] + (r * Split<T>::PARTS) * p.padded + c, p.padded, v);
+  put_eight<T>(p.dst[which] + r * p.padded + c, v);
 }
 
-// da and db, rounded (in parts): g [m][PARTS][2 hp], da at 0 .., db at hp .., zeros behind h; and the
+// da and db, rounded to T: g [m][2 hp], da at 0 .., db at hp .., zeros behind h; and the
 // column sums of every `rows` rows, sums [tiles of rows][2 h] (NULL: not wanted).  8
 // neighbouring columns of a row to a thread; ALIGNED: rows begin at 16 bytes.  HBM-bound.
 constexpr int kGradAcross = 32;  // threads side by side
@@ -89,7 +59,7 @@ int grad_rows(int64_t m, int64_t hp) {
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256)
     gated_grad_kernel(const T *__restrict__ dy, const void *__restrict__ ab, int64_t m, int64_t h, int act,
-                      int64_t hp, int rows, typename Split<T>::P *__restrict__ g,
+                      int64_t hp, int rows, T *__restrict__ g,
                       float *__restrict__ sums) {
   const Kept<T> kept(ab, m, h);
   constexpr int kDown = 256 / kGradAcross;
@@ -125,8 +95,8 @@ __global__ void __launch_bounds__(256)
         sa[i] += av[i];
         sb[i] += bv[i];
       }
-      put_chunk<T>(g + r * Split<T>::PARTS * 2 * hp + c, 2 * hp, av);
-      put_chunk<T>(g + r * Split<T>::PARTS * 2 * hp + hp + c, 2 * hp, bv);
+      put_eight<T>(g + r * 2 * hp + c, av);
+      put_eight<T>(g + r * 2 * hp + hp + c, bv);
     }
   }
   if (sums == nullptr) return;
@@ -337,7 +307,7 @@ struct Shape {
 // launch that adds them up costs more than they save.
 template <typename C> int slices_of(const Shape &s) {
   const int64_t tiles = tiles_of<C>(s.m, s.n), steps = ceil_div(s.k, C::BK);
-  int64_t z = tiles >= kCUs ? 1 : 2 * kCUs / tiles;
+  int64_t z = tiles >= kCUs * 3 / 4 ? 1 : 2 * kCUs / tiles;
   if (z > steps / 8) z = steps / 8;
   if (z < 1) z = 1;
   return (int)ceil_div(steps, ceil_div(steps, z));
@@ -408,7 +378,7 @@ int product(GemmArgs g, float *part, hipStream_t s) {
 
 // Whether the matrix kernel reads the user's rows as they are.
 template <typename T> bool reads_plain(int64_t k, const void *x, const void *wg, const void *wu) {
-  return Split<T>::PARTS == 1 && k % 8 == 0 && at16(x) && at16(wg) && at16(wu);
+  return sizeof(T) == 4 || (k % 8 == 0 && at16(x) && at16(wg) && at16(wu));
 }
 
 struct Problem {
@@ -425,27 +395,24 @@ template <typename T> bool takes_few(const Problem &p) {
   return sizeof(T) == 4 ? groups <= 896 : p.m <= 64 || groups <= kCUs;
 }
 
-size_t packed_bytes(int64_t rows, int64_t padded, int parts) {
-  return align_up((size_t)rows * padded * parts * 2);
-}
-
 // x and the weights as the matrix kernel reads them: as they are, or laid out anew in ws.
 template <typename T> struct Rows {
-  typedef typename Split<T>::P P;
-  static constexpr int PARTS = Split<T>::PARTS;
   Operand x, wg, wu;
+  int32_t k;  // columns
   static size_t bytes(const Problem &p) {
-    const int64_t kp = up8(p.k);
-    return packed_bytes(p.m, kp, PARTS) + 2 * packed_bytes(p.h, kp, PARTS);
+    if (sizeof(T) == 4) return 0;
+    const size_t row = up8(p.k) * sizeof(T);
+    return align_up(p.m * row) + 2 * align_up(p.h * row);
   }
   int make(const Problem &p, const void *x0, const void *wg0, const void *wu0, Carver &c, hipStream_t s) {
-    const int64_t kp = up8(p.k);
-    if (reads_plain<T>(p.k, x0, wg0, wu0)) {
+    const bool plain = reads_plain<T>(p.k, x0, wg0, wu0);
+    k = (int32_t)(plain ? p.k : up8(p.k));
+    if (plain) {
       x.p = x0;
       wg.p = wg0;
       wu.p = wu0;
     } else {
-      P *xp = c.take<P>(p.m * kp * PARTS), *gp = c.take<P>(p.h * kp * PARTS), *up = c.take<P>(p.h * kp * PARTS);
+      T *xp = c.take<T>(p.m * k), *gp = c.take<T>(p.h * k), *up = c.take<T>(p.h * k);
       PackArgs<T> a;
       a.src[0] = static_cast<const T *>(x0);
       a.src[1] = static_cast<const T *>(wg0);
@@ -453,26 +420,25 @@ template <typename T> struct Rows {
       a.dst[0] = xp;
       a.dst[1] = gp;
       a.dst[2] = up;
-      a.end[0] = p.m * (kp / 8);
-      a.end[1] = a.end[0] + p.h * (kp / 8);
-      a.end[2] = a.end[1] + p.h * (kp / 8);
+      a.end[0] = p.m * (k / 8);
+      a.end[1] = a.end[0] + p.h * (k / 8);
+      a.end[2] = a.end[1] + p.h * (k / 8);
       a.cols = p.k;
-      a.padded = kp;
+      a.padded = k;
       hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((uint32_t)ceil_div(a.end[2], 256)), dim3(256), 0, s, a);
       SSC_LAUNCH_CHECK("pack_rows_kernel");
       x.p = xp;
       wg.p = gp;
       wu.p = up;
     }
-    x.ld = wg.ld = wu.ld = kp * PARTS;
-    x.part = wg.part = wu.part = (int32_t)kp;
+    x.ld = wg.ld = wu.ld = k;
     x.second = wg.second = wu.second = 0x7FFFFFFF;
     return SSC_OK;
   }
 };
 
 template <typename T> size_t forward_bytes(const Problem &p) {
-  return takes_few<T>(p) ? 256 : Rows<T>::bytes(p);
+  return takes_few<T>(p) ? 256 : 256 + Rows<T>::bytes(p);
 }
 
 template <typename T, bool ALIGNED> void few_rows(const GemmArgs &g, hipStream_t s) {
@@ -510,7 +476,7 @@ int forward(const Problem &p, const void *x, const void *wg, const void *wu, con
   Rows<T> rows = {};
   const int rc = rows.make(p, x, wg, wu, c, s);
   if (rc != SSC_OK) return rc;
-  g.k = (int32_t)up8(p.k);
+  g.k = rows.k;
   g.a = rows.x;
   g.a.rows = p.m;
   g.b = rows.wg;
@@ -525,17 +491,15 @@ int forward(const Problem &p, const void *x, const void *wg, const void *wu, con
 }
 
 template <typename T> struct Backward {
-  typedef typename Split<T>::P P;
-  static constexpr int PARTS = Split<T>::PARTS;
   int64_t hp;  // columns of da and of db in g: a multiple of every tile's k
   int rows;    // of a workgroup of the pass that makes g
-  P *g;
+  T *g;
   float *sums, *part;
   size_t used;
   Backward(const Problem &p, void *ws) {
     hp = ceil_div(p.h, 64) * 64;
     Carver c(ws);
-    g = c.take<P>(p.m * PARTS * 2 * hp);
+    g = c.take<T>(p.m * 2 * hp);
     rows = grad_rows(p.m, hp);
     sums = c.take<float>(ceil_div(p.m, rows) * 2 * p.h);
     // the slices of the two products, one after the other
@@ -553,7 +517,6 @@ template <typename T>
 int backward(const Problem &p, const void *x, const void *wg, const void *wu, int act, const void *kept,
              const void *dy, void *dx, void *dwg, void *dwu, void *dbg, void *dbu,
              void *ws, hipStream_t s) {
-  constexpr int PARTS = Split<T>::PARTS;
   const Backward<T> w(p, ws);
   const bool biases = dbg != nullptr || dbu != nullptr;
   const dim3 tiles((uint32_t)ceil_div(p.m, w.rows), (uint32_t)ceil_div(w.hp, kGradAcross * 8));
@@ -578,8 +541,7 @@ int backward(const Problem &p, const void *x, const void *wg, const void *wu, in
   if (rc != SSC_OK) return rc;
   Operand grad = {};
   grad.p = w.g;
-  grad.ld = PARTS * 2 * w.hp;
-  grad.part = (int32_t)(2 * w.hp);
+  grad.ld = 2 * w.hp;
   grad.second = 0x7FFFFFFF;
   GemmArgs g = {};
   g.n = p.k;
@@ -589,7 +551,7 @@ int backward(const Problem &p, const void *x, const void *wg, const void *wu, in
     g.a.rows = p.m;
     g.b = rows.wg;
     g.b.q = rows.wu.p;
-    g.b.rows = up8(p.k);
+    g.b.rows = rows.k;
     g.b.second = (int32_t)w.hp;
     g.b.deep = (int32_t)p.h;
     g.m = p.m;
@@ -604,7 +566,7 @@ int backward(const Problem &p, const void *x, const void *wg, const void *wu, in
     g.a.rows = 2 * w.hp;
     g.a.deep = (int32_t)p.m;
     g.b = rows.x;
-    g.b.rows = up8(p.k);
+    g.b.rows = rows.k;
     g.b.deep = (int32_t)p.m;
     g.m = 2 * w.hp;
     g.k = (int32_t)p.m;

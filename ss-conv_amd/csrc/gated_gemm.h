@@ -5,12 +5,14 @@
 // on 16-bit matrix instructions.  An operand lies in memory either with k along its rows or as
 // the transpose, with k down the columns; LDS reads that transpose blocks of 4 x 16 elements
 // give the matrix instruction the same registers from either, so nothing is ever laid out anew.
-// float operands come as three bfloat16 parts a = a0 + a1 + a2 (each the rounding of what the
-// parts before it leave: 24 bits in all), laid one behind another in a row, and six of the nine
-// products of parts are taken: a0 b0, a0 b1, a1 b0, a1 b1, a0 b2, a2 b0.  What is left out is
-// below 2^-23 of |a||b|, and bfloat16 has the exponents of float, so no scaling is needed.
+// 16-bit elements go from memory straight to LDS.  Floats come by way of registers, where each is cut
+// into three bfloat16 parts a = a0 + a1 + a2 (24 bits in all), and six of the nine products of
+// parts are taken: a0 b0, a0 b1, a1 b0, a1 b1, a0 b2, a2 b0.  What is left out is below 2^-21 of
+// |a||b|, and bfloat16 has the exponents of float, so no scaling is needed.
 #ifndef SSC_GATED_GEMM_H_
 #define SSC_GATED_GEMM_H_
+
+#include <type_traits>
 
 #include "elem.h"
 
@@ -42,17 +44,16 @@ enum Epilogue {
 //   k along its rows:  p[row * ld + k], with a second array (kGated) for every other run of rows
 //   k down its columns: p[k * ld + row], and from k = `second` on q[(k - second) * ld + row];
 //                       each array has `deep` values of k, the rest count as zero
-// Parts (float operands) lie `part` elements apart.
 struct Operand {
   const void *p, *q;
   int64_t rows, ld;
-  int32_t part, deep, second;
+  int32_t deep, second;
 };
 
 struct GemmArgs {
   Operand a, b;
   int64_t m, n;           // of the results; kGated: n counts the hidden columns
-  int32_t k;              // a multiple of 8 (k along rows), of the tile's (k down columns)
+  int32_t k;              // 16 bits with k along rows: a multiple of 8
   int32_t kslice;         // values of k in a slice (kPartial), a multiple of the tile's
   int32_t tiles_m, tiles_n;
   // kStore, kPartial: rows from `second` on are those of out2; out and out2 have `each` rows
@@ -130,13 +131,13 @@ template <int R, int BK, int W, bool TR> struct Side {
           rows > 0 ? (int)(rows * o.ld * 2) : 0, 0x00020000);
     }
   }
-  template <bool LAST>
-  __device__ __forceinline__ void load(const Operand &, int k0, int k_end, int skip, int w, char *to) {
-    const int o = k0 + kc < k_end ? off : 0x7FFFFFFF;  // (what lies behind the slice counts as zero)
+  __device__ __forceinline__ void load(const Operand &, int k0, int k_end, int w, char *to) {
+    // (what lies behind the slice counts as zero; the whole offset is the lane's, which is the one
+    // that the resource's size is held against)
+    const int o = k0 + kc < k_end ? off + k0 * 2 : 0x7FFFFFFF;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs[i], (lds_ptr)(to + (i * W + w) * 1024), 16, o,
-                                               (k0 + skip) * 2, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs[i], (lds_ptr)(to + (i * W + w) * 1024), 16, o, 0, 0, 0);
   }
   template <typename F>
   static __device__ __forceinline__ F block(const char *tile, int row0, int kk, int lane) {
@@ -178,22 +179,18 @@ template <int R, int BK, int W> struct Side<R, BK, W, true> {
       off[i] = r0 + c < o.rows ? kr * row + c * 2 : 0x7FFFFFFF;
     }
   }
-  // One part of the next BK values of k; with the last part the step is done.
-  template <bool LAST>
-  __device__ __forceinline__ void load(const Operand &o, int, int, int skip, int w, char *to) {
+  // The next BK values of k.
+  __device__ __forceinline__ void load(const Operand &o, int, int, int w, char *to) {
     const int there = left < BK ? (int)left : BK;
     const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)cur, 0,
                                                       there > 0 ? (there - 1) * row + rest : 0, 0x00020000);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(to + (i * W + w) * 1024), 16, off[i],
-                                               skip * 2, 0, 0);
-    if constexpr (LAST) {
-      k += BK;
-      const bool turn = k == o.second;
-      cur = turn ? next : cur + (int64_t)BK * row;
-      left = turn ? (int64_t)o.deep : left - BK;
-    }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(to + (i * W + w) * 1024), 16, off[i], 0, 0, 0);
+    k += BK;
+    const bool turn = k == o.second;
+    cur = turn ? next : cur + (int64_t)BK * row;
+    left = turn ? (int64_t)o.deep : left - BK;
   }
   template <typename F>
   static __device__ __forceinline__ F block(const char *tile, int row0, int kk, int lane) {
@@ -207,6 +204,118 @@ template <int R, int BK, int W> struct Side<R, BK, W, true> {
           tile + k * (R * 2) + (((col >> 3) ^ swizzle(k)) << 4) + (col & 4) * 2));
     }
     return __builtin_bit_cast(F, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// The same for floats, 8 of them to a thread at a time: fetched into registers one step before they
+// are cut into parts and stored to LDS, so that the way from memory is covered by a whole step.
+__device__ __forceinline__ void cut_into_parts(const f32x4 (&v)[2], char *to, int stride) {
+  bf16x8 p[3];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = v[i / 4][i % 4];
+    // the first part is cut off, which no finite number overflows at, the others are rounded
+    const float a0 = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), r = x - a0;
+    const bf16 a1 = (bf16)r;
+    p[0][i] = __builtin_bit_cast(bf16, (unsigned short)(__float_as_uint(x) >> 16));
+    p[1][i] = a1;
+    p[2][i] = (bf16)(r - (float)a1);
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8 *>(to + k * stride) = p[k];
+}
+
+template <int R, int BK, int W, bool TR> struct FloatSide : Side<R, BK, W, false> {
+  static constexpr int kAcross = BK / 8, kRows = 64 / kAcross;  // rows that a wave's load covers
+  static constexpr int kLoads = R / (kRows * W);
+  static_assert(kLoads * kRows * W == R, "tile");
+  rsrc_t rs[kLoads];
+  f32x4 v[kLoads][2];
+  int off, kc, to;
+
+  template <int HALF>
+  __device__ __forceinline__ void init(const Operand &o, int64_t r0, int, int w, int lane) {
+    const int srow = lane / kAcross;
+    kc = lane % kAcross * 8;
+    off = (int)((srow * o.ld + kc) * 4);
+    to = (w * kRows + srow) * (BK * 2) + (((kc >> 3) ^ Side<R, BK, W, false>::swizzle(srow)) << 4);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int first = (i * W + w) * kRows;
+      const bool other = HALF > 0 && first % (2 * HALF) >= HALF;
+      const int64_t row = r0 + (HALF > 0 ? first / (2 * HALF) * HALF + first % HALF : first);
+      const int64_t rows = o.rows - row < kRows ? o.rows - row : kRows;
+      rs[i] = __builtin_amdgcn_make_buffer_rsrc(
+          (void *)((const char *)(other ? o.q : o.p) + (rows > 0 ? row : 0) * o.ld * 4), 0,
+          rows > 0 ? (int)(rows * o.ld * 4) : 0, 0x00020000);
+    }
+  }
+  __device__ __forceinline__ void fetch(const Operand &, int k0, int k_end) {
+    const int left = k_end - k0 - kc;  // values of this thread that exist
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v[i][h] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs[i], off + k0 * 4 + h * 16, 0, 0));
+        // (behind a row's end lies the next row)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][h][e] = h * 4 + e < left ? v[i][h][e] : 0.f;
+      }
+  }
+  __device__ __forceinline__ void store(char *tile, int stride) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) cut_into_parts(v[i], tile + i * (W * kRows * BK * 2) + to, stride);
+  }
+};
+
+template <int R, int BK, int W> struct FloatSide<R, BK, W, true> : Side<R, BK, W, true> {
+  typedef Side<R, BK, W, true> Base;  // (where it stands in memory, and the blocks' layout)
+  using Base::cur;
+  using Base::k;
+  using Base::left;
+  using Base::next;
+  using Base::rest;
+  using Base::row;
+  static constexpr int kAcross = R / 8, kLoads = BK * kAcross / (W * 64);
+  static_assert(kLoads * W * 64 == BK * kAcross, "tile");
+  f32x4 v[kLoads][2];
+  int at[kLoads], to[kLoads];
+
+  template <int HALF>
+  __device__ __forceinline__ void init(const Operand &o, int64_t r0, int k_begin, int w, int lane) {
+    const bool other = k_begin >= o.second;
+    k = k_begin;
+    left = o.deep - (other ? k_begin - o.second : k_begin);
+    next = (const char *)o.q + r0 * 4;
+    cur = (other ? next : (const char *)o.p + r0 * 4) + (o.deep - left) * o.ld * 4;
+    row = (int)o.ld * 4;
+    rest = (int)(o.ld - r0) * 4;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int id = (i * W + w) * 64 + lane, kr = id / kAcross, c = id % kAcross;
+      at[i] = kr * row + c * 32;
+      to[i] = kr * (R * 2) + ((c ^ Base::swizzle(kr)) << 4);
+    }
+  }
+  // (behind the last column lies the next row: columns of results that are not stored)
+  __device__ __forceinline__ void fetch(const Operand &o, int, int) {
+    const int there = left < BK ? (int)left : BK;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)cur, 0,
+                                                      there > 0 ? (there - 1) * row + rest : 0, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        v[i][h] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at[i] + h * 16, 0, 0));
+    k += BK;
+    const bool turn = k == o.second;
+    cur = turn ? next : cur + (int64_t)BK * row;
+    left = turn ? (int64_t)o.deep : left - BK;
+  }
+  __device__ __forceinline__ void store(char *tile, int stride) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) cut_into_parts(v[i], tile + to[i], stride);
   }
 };
 
@@ -376,27 +485,15 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
   constexpr int kCols = EPI == kGated ? C::BN / 2 : C::BN;
   constexpr int kHalf = C::kNi * 8;
   const int64_t n0 = (int64_t)tn * kCols;
-  typedef Side<C::BM, C::BK, C::kWaves, TA> SA;
-  typedef Side<C::BN, C::BK, C::kWaves, TB> SB;
+  constexpr bool kFloat = C::PARTS == 3;
+  typedef std::conditional_t<kFloat, FloatSide<C::BM, C::BK, C::kWaves, TA>, Side<C::BM, C::BK, C::kWaves, TA>> SA;
+  typedef std::conditional_t<kFloat, FloatSide<C::BN, C::BK, C::kWaves, TB>, Side<C::BN, C::BK, C::kWaves, TB>> SB;
   SA sa;
   SB sb;
   const int k_begin = EPI == kPartial ? (int)blockIdx.z * g.kslice : 0;
   const int k_end = EPI == kPartial && k_begin + g.kslice < g.k ? k_begin + g.kslice : g.k;
   sa.template init<0>(g.a, m0, k_begin, w, lane);
   sb.template init<EPI == kGated ? kHalf : 0>(g.b, n0, k_begin, w, lane);
-  // The loads of the step that begins at k0: called for one step after the other.
-  auto issue = [&](int k0, int s) {
-    char *st = lds + s * C::kStage;
-    if constexpr (C::PARTS == 3) {
-      sa.template load<false>(g.a, k0, k_end, 0, w, st);
-      sb.template load<false>(g.b, k0, k_end, 0, w, st + 3 * C::kABytes);
-      sa.template load<false>(g.a, k0, k_end, g.a.part, w, st + C::kABytes);
-      sb.template load<false>(g.b, k0, k_end, g.b.part, w, st + 3 * C::kABytes + C::kBBytes);
-    }
-    sa.template load<true>(g.a, k0, k_end, (C::PARTS - 1) * g.a.part, w, st + (C::PARTS - 1) * C::kABytes);
-    sb.template load<true>(g.b, k0, k_end, (C::PARTS - 1) * g.b.part, w,
-                           st + C::PARTS * C::kABytes + (C::PARTS - 1) * C::kBBytes);
-  };
 
   f32x4 acc[C::kNi][C::kMi];
 #pragma unroll
@@ -404,9 +501,15 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
 #pragma unroll
     for (int i = 0; i < C::kMi; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  if constexpr (C::PARTS == 1) {
+  if constexpr (!kFloat) {
     // Two stages in LDS and two sets of blocks in registers: while one set is multiplied the
     // next one is read, and a stage is loaded while the other one is read.
+    // The loads of the step that begins at k0: called for one step after the other.
+    auto issue = [&](int k0, int s) {
+      char *st = lds + s * C::kStage;
+      sa.load(g.a, k0, k_end, w, st);
+      sb.load(g.b, k0, k_end, w, st + C::kABytes);
+    };
     constexpr int kUnits = C::BK / 32;
     static_assert(kUnits == 2, "the sets change places once a stage");
     constexpr int kReads = C::kMi * (TA ? 2 : 1) + C::kNi * (TB ? 2 : 1), kMuls = C::kMi * C::kNi;
@@ -428,14 +531,26 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
       interleave<kReads, kMuls>();
     }
   } else {
-    // Two stages: while one is multiplied, the other one's loads are under way.
-    issue(k_begin, 0);
+    // Two stages in LDS: while one is multiplied the next step's floats are cut into the other one,
+    // and those of the step behind it are under way.
+    auto fetch = [&](int k0) {
+      sa.fetch(g.a, k0, k_end);
+      sb.fetch(g.b, k0, k_end);
+    };
+    auto store = [&](int s) {
+      sa.store(lds + s * C::kStage, C::kABytes);
+      sb.store(lds + s * C::kStage + 3 * C::kABytes, C::kBBytes);
+    };
+    fetch(k_begin);
+    store(0);
+    fetch(k_begin + C::BK);
     int s = 0;
     for (int k0 = k_begin; k0 < k_end; k0 += C::BK, s ^= 1) {
       __syncthreads();
-      if (k0 + C::BK < k_end) issue(k0 + C::BK, s ^ 1);
       Blocks<C> x;
       read_blocks<C, SA, SB>(lds + s * C::kStage, 0, wm, wn, x);
+      store(s ^ 1);  // (behind the last step these are zeros)
+      fetch(k0 + 2 * C::BK);
       multiply<C>(x, acc);
     }
   }
