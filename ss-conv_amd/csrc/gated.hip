@@ -140,17 +140,25 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Slices of a product added in order, rounded once.
-template <typename T>
+// Slices of a product added in order, rounded once: 4 neighbouring results of a thread where their
+// number allows it (V = 4), several slices' loads under way at a time.
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
     add_slices_kernel(const float *__restrict__ part, int slices, int64_t count, int64_t split,
                       T *__restrict__ out, T *__restrict__ out2) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
   if (i >= count) return;
-  float s = 0.f;
-  for (int z = 0; z < slices; ++z) s += part[z * count + i];
-  if (i < split) out[i] = (T)s;
-  else out2[i - split] = (T)s;
+  float s[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) s[e] = 0.f;
+#pragma unroll 8
+  for (int z = 0; z < slices; ++z) {
+    float v[V];
+    load_floats_once<float, V>(part + z * count + i, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] += v[e];
+  }
+  store_floats<T, V>(i < split ? out + i : out2 + (i - split), s);
 }
 
 // ---- few rows -------------------------------------------------------------------------------
@@ -303,11 +311,11 @@ struct Shape {
   int64_t m, n, k;
 };
 
-// Slices along k of a product with too few tiles to fill the chip; at least 8 steps each, or the
-// launch that adds them up costs more than they save.
+// Slices along k of a product with too few tiles to fill the chip, as many workgroups in all as fit on
+// it at a time; at least 8 steps each, or the launch that adds them up costs more than they save.
 template <typename C> int slices_of(const Shape &s) {
   const int64_t tiles = tiles_of<C>(s.m, s.n), steps = ceil_div(s.k, C::BK);
-  int64_t z = tiles >= kCUs * 3 / 4 ? 1 : 2 * kCUs / tiles;
+  int64_t z = tiles >= kCUs * 3 / 4 ? 1 : (C::kLds > 80 * 1024 ? 1 : 2) * kCUs / tiles;
   if (z > steps / 8) z = steps / 8;
   if (z < 1) z = 1;
   return (int)ceil_div(steps, ceil_div(steps, z));
@@ -317,19 +325,23 @@ template <typename C> int slices_of(const Shape &s) {
 // Forward: large tiles where they fill the chip, unless both projections are kept and k is short:
 // storing takes longer than multiplying then, and a CU holds only one large tile.  25600 rows ->
 // 1024, kept, bfloat16, large against middle tiles: k = 128 73 and 66 us, 256 82 and 81, 512 105 and
-// 110; floats, large against small: k = 128 195 and 148 us, 256 256 and 243, 512 387 and 403.
+// 110; 25437 -> 808, k = 128, float16 118 and 61.  Floats, large against small: 25600 -> 1024 kept,
+// k = 64 133 and 130, 128 154 and 162; 4096 -> 4096 kept, k = 64 86 and 69, 256 139 and 157.
 template <typename T> int forward_size(const Shape &s, bool kept) {
-  if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) >= kCUs && !(kept && s.k <= 384)) return 2;
+  const bool stores = kept && s.k <= (sizeof(T) == 4 ? 64 : 384);
+  if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) >= kCUs && !stores) return 2;
   return tiles_of<typename Tiles<T>::Middle>(s.m, s.n) >= kCUs ? 1 : 0;
 }
 // The products of the backward pass are sliced where tiles are few, so they fill the chip with any
 // of them; the tile's reuse counts for more the longer the product takes (times with the pass that
 // makes da and db).  bfloat16, large, middle, small: 25600 x 2048 (k) x 2048 293, 363, 377 us; 25600 x
 // 1024 (k) x 2048 207, 203, 283; 16384 x 512 (k) x 2048 101, 74, 78; 1024 x 2048 (k) x 2048 49, 45, 38.
+// Floats, large and small: 57304 x 1024 (k) x 128 110 and 138; 16384 x 512 (k) x 256 60 and 53; 1024 x
+// 2048 (k) x 1024 48 and 46; 300 x 8192 (k) x 2048 107 and 92.
 template <typename T> int product_size(const Shape &s) {
   const double work = (double)s.m * s.n * s.k;
   if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) >= kCUs * 3 / 4) return 2;
-  if (work >= (sizeof(T) == 4 ? 2e10 : 8e10)) return 2;
+  if (work >= (sizeof(T) == 4 ? 5.5e9 : 8e10)) return 2;
   return tiles_of<typename Tiles<T>::Middle>(s.m, s.n) >= kCUs || work >= 1.2e10 ? 1 : 0;
 }
 template <typename T> int slices_for(const Shape &s) {
@@ -370,8 +382,11 @@ int product(GemmArgs g, float *part, hipStream_t s) {
                                        : launch<typename S::Small, TA, TB, kPartial, float>(p, g.n, slices, s);
   if (rc != SSC_OK) return rc;
   const int64_t split = g.each * g.n, count = g.second < g.m ? 2 * split : split;
-  hipLaunchKernelGGL(add_slices_kernel<T>, dim3((uint32_t)ceil_div(count, 256)), dim3(256), 0, s, part,
-                     slices, count, split, static_cast<T *>(g.out), static_cast<T *>(g.out2));
+  const bool wide = split % 4 == 0 && at16(g.out) && at16(g.out2);
+  const dim3 grid((uint32_t)ceil_div(count, 256 * (wide ? 4 : 1)));
+  T *out = static_cast<T *>(g.out), *out2 = static_cast<T *>(g.out2);
+  if (wide) hipLaunchKernelGGL((add_slices_kernel<T, 4>), grid, dim3(256), 0, s, part, slices, count, split, out, out2);
+  else hipLaunchKernelGGL((add_slices_kernel<T, 1>), grid, dim3(256), 0, s, part, slices, count, split, out, out2);
   SSC_LAUNCH_CHECK("add_slices_kernel");
   return SSC_OK;
 }
