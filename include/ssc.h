@@ -939,7 +939,8 @@ int ssc_groupnorm_bwd(int32_t dtype, const void *x, const void *dy /* [n,c] */, 
  * taken in parts (six bfloat16 products, 24 bits), sums are float; a float infinity in x or the
  * weights comes out as NaN (infinity times a part that is zero).
  * ssc_gated_bwd: dx [m,k], dw_gate, dw_up [h,k] (both or none), db_gate, db_up [h], each NULL
- * where it is not wanted.  With m = 0 nothing is written.  m <= 2^24, k and h <= 2^21. */
+ * where it is not wanted.  With m = 0 nothing is written.  m <= 2^24, k and h <= 2^21; 16-bit x and
+ * weights whose rows are multiples of 16 bytes begin at 16 bytes. */
 size_t ssc_gated_fwd_workspace_bytes(int32_t dtype, int64_t m, int64_t k, int64_t h);
 size_t ssc_gated_kept_bytes(int32_t dtype, int64_t m, int64_t h);
 int ssc_gated_fwd(int32_t dtype, const void *x, int64_t m, int64_t k, const void *w_gate,

@@ -292,8 +292,8 @@ __global__ void __launch_bounds__(kThreads) adamw_values_kernel(const Table<Entr
         mv[j] = m_value((int)(int8_t)(mc >> (8 * j)), mq);
         vv[j] = v_value((int)(uint8_t)(vc >> (8 * j)), vq);
       }
-      if (mo) store_floats<float, kPer>(mo + at, mv);
-      if (vo) store_floats<float, kPer>(vo + at, vv);
+      if (mo) store_floats_once<float, kPer>(mo + at, mv);
+      if (vo) store_floats_once<float, kPer>(vo + at, vv);
     } else {
 #pragma unroll
       for (int j = 0; j < kPer; ++j)

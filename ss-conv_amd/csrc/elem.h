@@ -94,6 +94,25 @@ __device__ __forceinline__ float sigmoid_of(float z) {
   return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
 
+// The normal distribution function c of z, and e = exp(-z^2 / 2), by formula 7.1.26 of Abramowitz
+// and Stegun, Handbook of Mathematical Functions: erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 +
+// p x), off by at most 1.5e-7.  One exponential and one reciprocal serve value and slope, where the
+// library's erf and another exponential take three times the instructions (norm of 300000 x 256
+// bfloat16 with gelu, the writing pass 102 -> 75 us, the backward pass' sums 170 -> 132), and below
+// zero nothing cancels.
+__device__ __forceinline__ float normal_cdf(float z, float &e) {
+  const float x = fabsf(z) * 0.70710678f;
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+  e = __expf(-x * x);
+  float p = 1.061405429f;
+  p = p * t - 1.453152027f;
+  p = p * t + 1.421413741f;
+  p = p * t - 0.284496736f;
+  p = p * t + 0.254829592f;
+  const float tail = 0.5f * p * t * e;
+  return z < 0.f ? tail : 1.f - tail;
+}
+
 // f(z) of V values; `kind` is the same for a whole launch, so the branch is uniform.
 template <int V>
 __device__ __forceinline__ void activate(int kind, const float *z, float *f) {
@@ -116,7 +135,10 @@ __device__ __forceinline__ void activate(int kind, const float *z, float *f) {
       break;
     case SSC_ACT_GELU:
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = 0.5f * z[i] * (1.f + erff(z[i] * 0.70710678f));
+      for (int i = 0; i < V; ++i) {
+        float e;
+        f[i] = z[i] * normal_cdf(z[i], e);
+      }
       break;
     default:
 #pragma unroll
@@ -160,9 +182,10 @@ __device__ __forceinline__ void activate_slope(int kind, const float *z, float *
     case SSC_ACT_GELU:
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float c = 0.5f * (1.f + erff(z[i] * 0.70710678f));
+        float e;
+        const float c = normal_cdf(z[i], e);
         f[i] = z[i] * c;
-        d[i] = c + z[i] * __expf(-0.5f * z[i] * z[i]) * 0.39894228f;
+        d[i] = c + z[i] * e * 0.39894228f;
       }
       break;
     default:

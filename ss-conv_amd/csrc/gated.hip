@@ -391,10 +391,8 @@ int product(GemmArgs g, float *part, hipStream_t s) {
   return SSC_OK;
 }
 
-// Whether the matrix kernel reads the user's rows as they are.
-template <typename T> bool reads_plain(int64_t k, const void *x, const void *wg, const void *wu) {
-  return sizeof(T) == 4 || (k % 8 == 0 && at16(x) && at16(wg) && at16(wu));
-}
+// Whether the matrix kernel reads the user's rows as they are (16-bit ones begin at 16 bytes then).
+template <typename T> bool reads_plain(int64_t k) { return sizeof(T) == 4 || k % 8 == 0; }
 
 struct Problem {
   int64_t m, k, h;
@@ -415,12 +413,12 @@ template <typename T> struct Rows {
   Operand x, wg, wu;
   int32_t k;  // columns
   static size_t bytes(const Problem &p) {
-    if (sizeof(T) == 4) return 0;
+    if (reads_plain<T>(p.k)) return 0;
     const size_t row = up8(p.k) * sizeof(T);
     return align_up(p.m * row) + 2 * align_up(p.h * row);
   }
   int make(const Problem &p, const void *x0, const void *wg0, const void *wu0, Carver &c, hipStream_t s) {
-    const bool plain = reads_plain<T>(p.k, x0, wg0, wu0);
+    const bool plain = reads_plain<T>(p.k);
     k = (int32_t)(plain ? p.k : up8(p.k));
     if (plain) {
       x.p = x0;
@@ -597,7 +595,8 @@ int backward(const Problem &p, const void *x, const void *wg, const void *wu, in
 // What 32-bit offsets inside a few rows allow.
 constexpr int64_t kMostAlong = 1 << 24;
 
-int check(int32_t dtype, int64_t m, int64_t k, int64_t h, int32_t act) {
+int check(int32_t dtype, int64_t m, int64_t k, int64_t h, int32_t act, const void *x, const void *wg,
+          const void *wu) {
   SSC_CHECK(dtype_ok(dtype), SSC_EINVAL, "element type %d", dtype);
   SSC_CHECK(m >= 0 && k >= 1 && h >= 1, SSC_EINVAL, "%lld rows, widths %lld and %lld", (long long)m,
             (long long)k, (long long)h);
@@ -605,6 +604,9 @@ int check(int32_t dtype, int64_t m, int64_t k, int64_t h, int32_t act) {
             "%lld rows, widths %lld and %lld: at most %lld and %lld", (long long)m, (long long)k,
             (long long)h, (long long)kMostAlong, (long long)(kMostAlong / 8));
   SSC_CHECK(pointwise_act_ok(act), SSC_EINVAL, "activation %d", act);
+  SSC_CHECK(m == 0 || (x && wg && wu), SSC_EINVAL, "NULL pointer");
+  SSC_CHECK(m == 0 || dtype == SSC_F32 || k % 8 != 0 || (at16(x) && at16(wg) && at16(wu)), SSC_EINVAL,
+            "x and the weights begin at 16 bytes where their rows are multiples of 16 bytes");
   return SSC_OK;
 }
 
@@ -627,10 +629,10 @@ extern "C" int ssc_gated_fwd(int32_t dtype, const void *x, int64_t m, int64_t k,
                              const void *w_up, int64_t h, const void *b_gate, const void *b_up,
                              int32_t act, void *y, void *kept, void *ws, size_t ws_bytes,
                              ssc_stream_t stream) {
-  const int rc = check(dtype, m, k, h, act);
+  const int rc = check(dtype, m, k, h, act, x, w_gate, w_up);
   if (rc != SSC_OK) return rc;
   if (m == 0) return SSC_OK;
-  SSC_CHECK(x && w_gate && w_up && y, SSC_EINVAL, "NULL pointer");
+  SSC_CHECK(y, SSC_EINVAL, "NULL pointer");
   SSC_CHECK(at16(kept), SSC_EINVAL, "what is kept begins at 16 bytes");
   SSC_CHECK(ws != nullptr && ws_bytes >= ssc_gated_fwd_workspace_bytes(dtype, m, k, h), SSC_EWORKSPACE,
             "workspace of %zu bytes, %zu are needed", ws_bytes,
@@ -652,10 +654,10 @@ extern "C" int ssc_gated_bwd(int32_t dtype, const void *x, int64_t m, int64_t k,
                              const void *w_up, int64_t h, int32_t act, const void *kept, const void *dy,
                              void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *ws,
                              size_t ws_bytes, ssc_stream_t stream) {
-  const int rc = check(dtype, m, k, h, act);
+  const int rc = check(dtype, m, k, h, act, x, w_gate, w_up);
   if (rc != SSC_OK) return rc;
   if (m == 0) return SSC_OK;
-  SSC_CHECK(x && w_gate && w_up && kept && dy && (dw_gate == nullptr) == (dw_up == nullptr), SSC_EINVAL,
+  SSC_CHECK(kept && dy && (dw_gate == nullptr) == (dw_up == nullptr), SSC_EINVAL,
             "NULL pointer");
   SSC_CHECK(at16(kept), SSC_EINVAL, "what is kept begins at 16 bytes");
   SSC_CHECK(ws != nullptr && ws_bytes >= ssc_gated_bwd_workspace_bytes(dtype, m, k, h), SSC_EWORKSPACE,

@@ -185,11 +185,24 @@ __device__ __forceinline__ S block_sum(S v, S *lds) {
   return t;
 }
 
+// How the threads of a workgroup that adds up pieces lie on the `per` channels of a group and on the
+// pieces: channels side by side (in turns of `tx`), `ty` pieces at a time.
+struct GroupLay {
+  int tx, ty, row, cx;
+  __device__ GroupLay(const Norm &a) {
+    const int threads = (int)blockDim.x;
+    tx = a.per < threads ? a.per : threads;
+    ty = threads / tx;
+    row = (int)threadIdx.x / tx;
+    cx = (int)threadIdx.x - row * tx;
+  }
+};
+
 // mean and rstd of group blockIdx.x % groups of cloud blockIdx.x / groups, from the channels'
 // means and squared deviations in the pieces of the cloud.  Sums over at most a few thousand
 // numbers, in double: their cost does not show.
 __global__ void __launch_bounds__(1024) norm_finish_kernel(const Norm a) {
-  __shared__ double lds[16];
+  __shared__ double lds[3][16];
   const int b = blockIdx.x / a.groups, g = blockIdx.x - b * a.groups;
   const int64_t s = cloud_begin(a, b), e = cloud_begin(a, b + 1);
   if (s >= e) {
@@ -199,26 +212,38 @@ __global__ void __launch_bounds__(1024) norm_finish_kernel(const Norm a) {
     }
     return;
   }
-  const int64_t k0 = s / a.rows, k1 = (e - 1) / a.rows;
-  const float2 *p = a.partial + (k0 + b) * a.c + (int64_t)g * a.per;
+  const int k0 = (int)(s / a.rows), pieces = (int)((e - 1) / a.rows) - k0 + 1;
+  const float2 *p = a.partial + ((int64_t)k0 + b) * a.c + (int64_t)g * a.per;
   const double shift = p[0].x;
-  double n = 0, s1 = 0, s2 = 0;
-  const int64_t items = (k1 - k0 + 1) * a.per;
-  for (int64_t i = threadIdx.x; i < items; i += blockDim.x) {
-    const int64_t k = i / a.per;
-    const float2 v = p[k * a.c + (i - k * a.per)];
-    const int64_t kb = (k0 + k) * a.rows, ke = kb + a.rows;
-    const double rows = (double)((ke < e ? ke : e) - (kb > s ? kb : s));
-    const double d = (double)v.x - shift;
-    n += rows;
-    s1 += rows * d;
-    s2 += (double)v.y + rows * d * d;
+  double sums[3] = {0, 0, 0};  // rows, of means, of squared deviations
+  const GroupLay lay(a);
+  if (lay.row < lay.ty)
+    for (int c = lay.cx; c < a.per; c += lay.tx) {
+#pragma unroll 4
+      for (int k = lay.row; k < pieces; k += lay.ty) {
+        const float2 v = p[(int64_t)k * a.c + c];
+        const int64_t kb = ((int64_t)k0 + k) * a.rows, ke = kb + a.rows;
+        const double rows = (double)(int)((ke < e ? ke : e) - (kb > s ? kb : s));
+        const double d = (double)v.x - shift;
+        sums[0] += rows;
+        sums[1] += rows * d;
+        sums[2] += (double)v.y + rows * d * d;
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sums[i] += __shfl_xor(sums[i], d, 64);
+    if ((threadIdx.x & 63) == 0) lds[i][threadIdx.x >> 6] = sums[i];
   }
-  n = block_sum(n, lds);
-  s1 = block_sum(s1, lds);
-  s2 = block_sum(s2, lds);
+  __syncthreads();
   if (threadIdx.x == 0) {
-    const double d = s1 / n, var = s2 / n - d * d;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      sums[i] = 0;
+      for (int w = 0; w < (int)(blockDim.x >> 6); ++w) sums[i] += lds[i][w];
+    }
+    const double d = sums[1] / sums[0], var = sums[2] / sums[0] - d * d;
     a.mean[blockIdx.x] = (float)(shift + d);
     a.rstd[blockIdx.x] = (float)(1.0 / sqrt((var < 0 ? 0 : var) + (double)a.eps));
   }
@@ -372,32 +397,41 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const Norm a) {
   __shared__ float total[16];
   const int b = blockIdx.x / a.groups, g = blockIdx.x - b * a.groups;
   const int64_t s = cloud_begin(a, b), e = cloud_begin(a, b + 1);
-  const int64_t k0 = s / a.rows, k1 = s < e ? (e - 1) / a.rows + 1 : k0;
-  const int threads = blockDim.x;
+  const int k0 = (int)(s / a.rows), pieces = s < e ? (int)((e - 1) / a.rows) - k0 + 1 : 0;
+  const float2 *p = a.partial + ((int64_t)k0 + b) * a.c + (int64_t)g * a.per;
+  const GroupLay lay(a);
   float t1 = 0.f, t2 = 0.f;
-  for (int c0 = 0; c0 < a.per; c0 += threads) {  // (one turn unless a group has over 1024 channels)
-    const int tx = a.per - c0 < threads ? a.per - c0 : threads, ty = threads / tx;
-    const int row = threadIdx.x / tx, cx = threadIdx.x - row * tx;
-    const int64_t ch = (int64_t)g * a.per + c0 + cx;
+  for (int c0 = 0; c0 < a.per; c0 += lay.tx) {  // (one turn unless a group has over 1024 channels)
+    const int c = c0 + lay.cx;
+    const bool in = lay.row < lay.ty && c < a.per;
     float s1 = 0.f, s2 = 0.f;
-    if (row < ty)
-      for (int64_t k = k0 + row; k < k1; k += ty) {
-        const float2 v = a.partial[(k + b) * a.c + ch];
+    if (in) {
+#pragma unroll 4
+      for (int k = lay.row; k < pieces; k += lay.ty) {
+        const float2 v = p[(int64_t)k * a.c + c];
         s1 += v.x;
         s2 += v.y;
       }
+    }
     __syncthreads();
     lds[threadIdx.x] = make_float2(s1, s2);
     __syncthreads();
-    if (row == 0) {
-      for (int y = 1; y < ty; ++y) {
-        s1 += lds[y * tx + cx].x;
-        s2 += lds[y * tx + cx].y;
+    int half = 1;
+    while (half * 2 < lay.ty) half *= 2;
+    for (; half > 0 && lay.ty > 1; half >>= 1) {
+      if (lay.row < half && lay.row + half < lay.ty) {
+        const float2 v = lds[threadIdx.x], o = lds[threadIdx.x + half * lay.tx];
+        lds[threadIdx.x] = make_float2(v.x + o.x, v.y + o.y);
       }
-      a.sums[(int64_t)b * a.c + ch] = make_float2(s1, s2);
+      __syncthreads();
+    }
+    if (in && lay.row == 0) {
+      const int64_t ch = (int64_t)g * a.per + c;
+      const float2 v = lds[threadIdx.x];
+      a.sums[(int64_t)b * a.c + ch] = v;
       const float w = a.weight ? load_any(a.weight, ch, a.wtype) : 1.f;
-      t1 += w * s1;
-      t2 += w * s2;
+      t1 += w * v.x;
+      t2 += w * v.y;
     }
   }
   t1 = block_sum(t1, total);
@@ -595,11 +629,12 @@ __global__ void __launch_bounds__(kFewThreads) norm_few_backward_kernel(const No
 }
 
 // ---- host -----------------------------------------------------------------------------------
-// Rows of a chunk: enough that at most kChunksMost chunks are left, and at least 32, so that the
-// partial results stay small beside the rows.
-int64_t chunk_rows(int64_t n) {
-  const int64_t r = ceil_div(n, kChunksMost);
-  return r < 32 ? 32 : r;
+// Rows of a chunk: enough that at most kChunksMost chunks are left, that the partial results stay
+// small beside the rows, and that every thread of a workgroup has some (8 channels to a thread).
+int64_t chunk_rows(int64_t n, int c) {
+  const int64_t r = ceil_div(n, kChunksMost), across = ceil_div(c, 8);
+  const int64_t least = across < kThreads / 16 ? 2 * kThreads / across : 32;
+  return r < least ? least : r;
 }
 
 bool same_alignment(const void *a, const void *b, const void *c, size_t to) {
@@ -623,19 +658,29 @@ bool few(const Norm &a) {
   return a.per <= kFewThreads && a.n * a.per <= kFewMost && a.n * a.per <= kFewMean * a.clouds;
 }
 
+// Channels of a thread: 16 bytes of a row where rows and pointers allow it, 8 bytes, or one.
+template <typename T> int width(const Norm &a) {
+  constexpr int V = 16 / sizeof(T);
+  if (a.c % V == 0 && same_alignment(a.x, a.dy, a.out, 16)) return V;
+  return V == 8 && a.c % 4 == 0 && same_alignment(a.x, a.dy, a.out, 8) ? 4 : 1;
+}
+#define SSC_NORM_LAUNCH(KERNEL, V) \
+  hipLaunchKernelGGL((KERNEL<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a)
+#define SSC_NORM_WIDTHS(KERNEL)                                         \
+  if (v == 16 / (int)sizeof(T)) SSC_NORM_LAUNCH(KERNEL, 16 / sizeof(T)); \
+  else if (v == 4) SSC_NORM_LAUNCH(KERNEL, 4);                           \
+  else SSC_NORM_LAUNCH(KERNEL, 1)
+
 template <typename T> int forward(const Norm &a, hipStream_t s) {
   if (few(a)) {
     hipLaunchKernelGGL(norm_few_kernel<T>, dim3(a.clouds * a.groups), dim3(kFewThreads), 0, s, a);
     SSC_LAUNCH_CHECK("group norm, forward");
     return SSC_OK;
   }
-  constexpr int V = 16 / sizeof(T);
-  const bool wide = a.c % V == 0 && same_alignment(a.x, a.x, a.out, 16);
-  if (wide) hipLaunchKernelGGL((norm_stats_kernel<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a);
-  else hipLaunchKernelGGL((norm_stats_kernel<T, 1>), chunk_grid(a, 1), dim3(kThreads), 0, s, a);
+  const int v = width<T>(a);
+  SSC_NORM_WIDTHS(norm_stats_kernel);
   hipLaunchKernelGGL(norm_finish_kernel, dim3(a.clouds * a.groups), dim3(finish_threads(a)), 0, s, a);
-  if (wide) hipLaunchKernelGGL((norm_apply_kernel<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a);
-  else hipLaunchKernelGGL((norm_apply_kernel<T, 1>), chunk_grid(a, 1), dim3(kThreads), 0, s, a);
+  SSC_NORM_WIDTHS(norm_apply_kernel);
   SSC_LAUNCH_CHECK("group norm, forward");
   return SSC_OK;
 }
@@ -643,27 +688,25 @@ template <typename T> int forward(const Norm &a, hipStream_t s) {
 template <typename T> int backward(const Norm &a, hipStream_t s) {
   if (few(a)) {
     hipLaunchKernelGGL(norm_few_backward_kernel<T>, dim3(a.clouds * a.groups), dim3(kFewThreads), 0, s, a);
-    if (a.dweight || a.dbias)
-      hipLaunchKernelGGL(norm_params_kernel, dim3((uint32_t)ceil_div(a.c, 16)), dim3(kThreads), 0, s, a);
-    SSC_LAUNCH_CHECK("group norm, backward");
-    return SSC_OK;
+  } else {
+    const int v = width<T>(a);
+    SSC_NORM_WIDTHS(norm_sums_kernel);
+    hipLaunchKernelGGL(norm_reduce_kernel, dim3(a.clouds * a.groups), dim3(finish_threads(a)), 0, s, a);
+    if (a.out) {
+      SSC_NORM_WIDTHS(norm_dx_kernel);
+    }
   }
-  constexpr int V = 16 / sizeof(T);
-  const bool wide = a.c % V == 0 && same_alignment(a.x, a.dy, a.out, 16);
-  if (wide) hipLaunchKernelGGL((norm_sums_kernel<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a);
-  else hipLaunchKernelGGL((norm_sums_kernel<T, 1>), chunk_grid(a, 1), dim3(kThreads), 0, s, a);
-  hipLaunchKernelGGL(norm_reduce_kernel, dim3(a.clouds * a.groups), dim3(finish_threads(a)), 0, s, a);
   if (a.dweight || a.dbias)
     hipLaunchKernelGGL(norm_params_kernel, dim3((uint32_t)ceil_div(a.c, 16)), dim3(kThreads), 0, s, a);
-  if (a.out && wide) hipLaunchKernelGGL((norm_dx_kernel<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a);
-  else if (a.out) hipLaunchKernelGGL((norm_dx_kernel<T, 1>), chunk_grid(a, 1), dim3(kThreads), 0, s, a);
   SSC_LAUNCH_CHECK("group norm, backward");
   return SSC_OK;
 }
+#undef SSC_NORM_WIDTHS
+#undef SSC_NORM_LAUNCH
 
 size_t workspace(int64_t n, int32_t c, int32_t clouds, int32_t groups) {
   if (n <= 0) return 256;
-  const int64_t chunks = ceil_div(n, chunk_rows(n));
+  const int64_t chunks = ceil_div(n, chunk_rows(n, c));
   return align_up((size_t)(chunks + clouds) * c * sizeof(float2)) +
          align_up((size_t)clouds * c * sizeof(float2)) +
          align_up((size_t)clouds * groups * sizeof(float2));
@@ -692,7 +735,7 @@ Norm carve(int64_t n, int32_t c, int32_t clouds, int32_t groups, void *ws) {
   a.clouds = clouds;
   a.groups = groups;
   a.per = c / groups;
-  a.rows = (int32_t)chunk_rows(n);
+  a.rows = (int32_t)chunk_rows(n, c);
   Carver w(ws);
   a.partial = w.take<float2>((size_t)(ceil_div(n, a.rows) + clouds) * c);
   a.sums = w.take<float2>((size_t)clouds * c);

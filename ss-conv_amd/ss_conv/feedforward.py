@@ -40,6 +40,11 @@ class _GatedLinear(torch.autograd.Function):
                             dy.contiguous(), want) + (None,)
 
 
+def _at_16_bytes(t):
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """activation(x w_gate^T + b_gate) * (x w_up^T + b_up) for x [..., K] and weights [H, K].
 
@@ -61,8 +66,8 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
         pointwise.check_like(what, t, shape, (x.dtype,), x.device)
     if w_up is None:
         raise TypeError("w_up is missing")
-    rows = (x if x.dim() == 2 else x.reshape(-1, k)).contiguous()
-    w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+    rows = _at_16_bytes(x if x.dim() == 2 else x.reshape(-1, k))
+    w_gate, w_up = _at_16_bytes(w_gate), _at_16_bytes(w_up)
     b_gate, b_up = [None if t is None else t.contiguous() for t in (b_gate, b_up)]
     args = (rows, w_gate, w_up, b_gate, b_up)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
