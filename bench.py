@@ -74,6 +74,10 @@ def parse_args():
                     help="also time layers whose last group of 16 output columns would be alone "
                          "in its block of 64 (64->72, 128->136, 152->8, 128->16), with the "
                          "kernel's one-column-group form and without (table on stderr)")
+    ap.add_argument("--pointwise", action="store_true",
+                    help="also time a training step of two pointwise blocks (group norm, gated "
+                         "feed-forward, AdamW with moments in 32 bits and in 8) on the voxel rows "
+                         "of cfg2 (table on stderr)")
     ap.add_argument("--one-stream", action="store_true",
                     help="queue the index work (rulebooks, plans) on the convolutions' stream "
                          "instead of a second one: a step's kernels one after the other (for "
@@ -584,6 +588,48 @@ def thin_layer_table(torch, _ext, synth, dev, seed):
     print("\n".join(rows), file=sys.stderr)
 
 
+def pointwise_table(torch, synth, dev, seed, width=128, hidden=512, n=20, warm=3):
+    """A training step (forward, backward, AdamW) of two blocks x + down(gated(norm(x))) on the
+    voxel rows of the second configuration, clouds as Point2Voxel returns them."""
+    from ss_conv.feedforward import GatedFeedForward
+    from ss_conv.groupnorm import GroupNorm
+    from ss_conv.optim import AdamW
+    from ss_conv.sp_ops.tensor import SparseTensor
+    cfg = synth.CONFIGS["cfg2"]
+    pts, _, ids = synth.config_clouds("cfg2", seed)
+    idx = torch.from_numpy(synth.voxel_indices(pts, ids, cfg["grid"])).to(dev)
+    rows = idx.shape[0]
+    lines = []
+    for dtype in (torch.float32, torch.bfloat16):
+        for bits in (32, 8):
+            torch.manual_seed(seed)
+            net = torch.nn.Sequential(*[GatedFeedForward(width, hidden, GroupNorm(16, width), bias=True)
+                                        for _ in range(2)]).to(dev, dtype)
+            opt = AdamW(net.parameters(), lr=1e-3, state_bits=bits)
+            x = torch.randn(rows, width, device=dev).to(dtype)
+            target = torch.randn(rows, width, device=dev).to(dtype)
+
+            def step():
+                opt.zero_grad()
+                out = net(SparseTensor(x, idx, [cfg["grid"]] * 3, cfg["batch"]))
+                loss = (out.features - target).float().square().mean()
+                loss.backward()
+                opt.step()
+                return loss.detach()
+
+            losses = [step() for _ in range(warm)]
+            torch.cuda.synchronize()
+            a = time.perf_counter()
+            for _ in range(n):
+                losses.append(step())
+            torch.cuda.synchronize()
+            ms = (time.perf_counter() - a) * 1e3 / n
+            lines.append("%d rows, 2 blocks %d -> %d -> %d, %s, moments in %2d bits: %.3f ms a step, "
+                         "loss %.4f -> %.4f" % (rows, width, hidden, width, str(dtype)[6:], bits, ms,
+                                                float(losses[0]), float(losses[-1])))
+    print("\n".join(lines), file=sys.stderr)
+
+
 def backbone_table(torch, _ext, synth, dev, seed, n=5, warm=2):
     """Runs the backbone of the fourth configuration and prints one row per convolution
     stage: rows, pairs, flops, the MFMA kernel's time (HIP events around its launch) and
@@ -923,6 +969,8 @@ def main():
         backbone_table(torch, _ext, synth, dev, args.seed)
     if args.thin_layers:
         thin_layer_table(torch, _ext, synth, dev, args.seed)
+    if args.pointwise:
+        pointwise_table(torch, synth, dev, args.seed)
 
     if not args.no_cpu_baseline:
         w = conv.kernel().detach().permute(2, 3, 4, 1, 0).reshape(K, c_in, c_out).cpu().numpy()
