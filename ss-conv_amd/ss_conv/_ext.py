@@ -7,7 +7,6 @@ library the import fails, and without a GPU every call raises.
 """
 import array
 import ctypes
-import itertools
 import os
 import threading
 
@@ -1955,20 +1954,25 @@ def gated_backward(x, w_gate, w_up, act, kept, dy, want):
     return dx, dw_gate if want[1] else None, dw_up if want[2] else None, db_gate, db_up
 
 
-def adamw_table(columns):
+def adamw_table(columns, count):
     """An array of ssc_adamw_tensor, whose fields are eight words each, from the columns param,
-    grad, exp_avg, exp_avg_sq, scale, scale, numel, element type; addresses as integers."""
-    return array.array("q", itertools.chain.from_iterable(zip(*columns)))
+    grad, exp_avg, exp_avg_sq, scale, scale, numel, element type (None: zeros); addresses as
+    integers."""
+    table = array.array("q", bytes(64 * count))
+    for i, column in enumerate(columns):
+        if column is not None:
+            table[i::8] = array.array("q", column)
+    return table
 
 
 def adamw_step(columns, count, state_bits, lr, beta1, beta2, eps, weight_decay, step, stream):
-    table = adamw_table(columns)
+    table = adamw_table(columns, count)
     _check(_lib.ssc_adamw_step(table.buffer_info()[0], count, state_bits, lr, beta1, beta2, eps,
                                weight_decay, step, stream))
 
 
 def adamw_values(columns, count, stream):
-    table = adamw_table(columns)
+    table = adamw_table(columns, count)
     _check(_lib.ssc_adamw_values(table.buffer_info()[0], count, stream))
 
 

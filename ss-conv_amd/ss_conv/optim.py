@@ -143,8 +143,8 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.99
             grads[i] = _like(grads[i], p)
     columns = [map(torch.Tensor.data_ptr, x) for x in [params] + lists]
     if not eight:
-        columns += [itertools.repeat(0)] * 2
-    columns += [sizes, [_ext.ELEM[t] for t in kinds]]
+        columns += [None, None]
+    columns += [sizes, map(_ext.ELEM.__getitem__, kinds)]
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("an AdamW step cannot be captured into a graph: the number of the step "
                            "is an argument of its launch")
@@ -178,7 +178,7 @@ def state_values(exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, out=N
             # (a new tensor has the layout of the codes, a given one has to have it)
             _check_order(i, exp_avgs[i], (exp_avg_sqs[i], out[0][i], out[1][i]))
     columns = [map(torch.Tensor.data_ptr, x) for x in list(out) + moments]
-    columns += [sizes, itertools.repeat(0)]
+    columns += [sizes, None]
     _ext.call_on(exp_avgs[0], _ext.adamw_values, columns, count, _ext._raw_stream(dev.index))
     return tuple(out)
 
