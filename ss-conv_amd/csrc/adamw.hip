@@ -59,6 +59,7 @@ template <typename E, int N> struct Table {
   Consts k;
   int32_t count;
 };
+constexpr int64_t kBlocksMost = (int64_t(1) << 32) / kThreads - 1;  // a grid has fewer than 2^32 threads
 constexpr int kMost32 = 88, kMost8 = 64;
 static_assert(sizeof(Table<Entry32, kMost32>) <= 4096 && sizeof(Table<Entry8, kMost8>) <= 4096,
               "kernel arguments");
@@ -325,7 +326,7 @@ int launch_all(K kernel, const ssc_adamw_tensor *tensors, int32_t n, size_t mome
   int64_t blocks = 0;
   for (int32_t i = 0; i <= n; ++i) {
     const int64_t more = i < n ? ceil_div(tensors[i].numel, kChunk) : 0;
-    if (t.count > 0 && (i == n || t.count == N || blocks + more > 0x7FFFFFFF)) {
+    if (t.count > 0 && (i == n || t.count == N || blocks + more > kBlocksMost)) {
       hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kThreads), 0, s, t);
       SSC_LAUNCH_CHECK(name);
       t.count = 0;
@@ -364,7 +365,7 @@ extern "C" int ssc_adamw_step(const ssc_adamw_tensor *tensors, int32_t n_tensors
   SSC_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, SSC_EINVAL, "betas are in [0, 1)");
   for (int32_t i = 0; i < n_tensors; ++i) {
     const ssc_adamw_tensor &t = tensors[i];
-    SSC_CHECK(t.numel >= 0 && ceil_div(t.numel, kChunk) <= 0x7FFFFFFF, SSC_EINVAL,
+    SSC_CHECK(t.numel >= 0 && ceil_div(t.numel, kChunk) <= kBlocksMost, SSC_EINVAL,
               "tensor %d: bad number of elements", i);
     SSC_CHECK(t.dtype >= 0 && dtype_ok((int)t.dtype), SSC_EINVAL,
               "tensor %d: element type %lld", i, (long long)t.dtype);
@@ -393,7 +394,7 @@ extern "C" int ssc_adamw_values(const ssc_adamw_tensor *tensors, int32_t n_tenso
             "bad table of tensors");
   for (int32_t i = 0; i < n_tensors; ++i) {
     const ssc_adamw_tensor &t = tensors[i];
-    SSC_CHECK(t.numel >= 0 && ceil_div(t.numel, kChunk) <= 0x7FFFFFFF, SSC_EINVAL,
+    SSC_CHECK(t.numel >= 0 && ceil_div(t.numel, kChunk) <= kBlocksMost, SSC_EINVAL,
               "tensor %d: bad number of elements", i);
     SSC_CHECK(t.dtype == SSC_F32, SSC_EINVAL, "tensor %d: values are floats", i);
     SSC_CHECK(t.numel == 0 || ((!t.param || (t.exp_avg && t.exp_avg_scale)) &&

@@ -622,13 +622,15 @@ int check(int32_t dtype, int64_t m, int64_t k, int64_t h, int32_t act, const voi
 using namespace ssc;
 
 extern "C" size_t ssc_gated_fwd_workspace_bytes(int32_t dtype, int64_t m, int64_t k, int64_t h) {
+  if (m <= 0 || k <= 0 || h <= 0) return 256;  // (the calls refuse all but no rows)
   const Problem p = {m, k, h};
   return dtype == SSC_F32 ? forward_bytes<float>(p) : forward_bytes<f16>(p);
 }
 
 extern "C" size_t ssc_gated_kept_bytes(int32_t dtype, int64_t m, int64_t h) {
+  if (m <= 0 || h <= 0) return 16;
   const size_t bytes = dtype == SSC_F32 ? Kept<float>::bytes(m, h) : Kept<f16>::bytes(m, h);
-  return bytes > 0 ? bytes : 16;
+  return bytes;
 }
 
 extern "C" int ssc_gated_fwd(int32_t dtype, const void *x, int64_t m, int64_t k, const void *w_gate,
@@ -651,7 +653,7 @@ extern "C" int ssc_gated_fwd(int32_t dtype, const void *x, int64_t m, int64_t k,
 }
 
 extern "C" size_t ssc_gated_bwd_workspace_bytes(int32_t dtype, int64_t m, int64_t k, int64_t h) {
-  if (m <= 0) return 256;
+  if (m <= 0 || k <= 0 || h <= 0) return 256;
   const Problem p = {m, k, h};
   return dtype == SSC_F32 ? Backward<float>::bytes(p) : Backward<f16>::bytes(p);
 }

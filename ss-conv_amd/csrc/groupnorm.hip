@@ -44,6 +44,7 @@ struct Norm {
   void *dweight, *dbias;     // [c] or NULL
   int64_t n;
   int32_t c, clouds, groups, per, wtype, act, rows;  // rows: of a chunk
+  int32_t first;             // a launch with a workgroup to a cloud's group: the first one's number
   float eps;
 };
 
@@ -138,7 +139,9 @@ __global__ void __launch_bounds__(kThreads) norm_stats_kernel(const Norm a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float d = s1[i] * inv;
-      lds[threadIdx.x * V + i] = make_float2(first[i] + d, fmaxf(s2[i] - s1[i] * d, 0.f));
+      // (squares that pass float stay infinite, as the variance is then, and NaN stays NaN)
+      const float dev = s2[i] < __builtin_inff() ? fmaxf(s2[i] - s1[i] * d, 0.f) : s2[i];
+      lds[threadIdx.x * V + i] = make_float2(first[i] + d, dev);
     }
     counts[threadIdx.x] = count;
     __syncthreads();
@@ -198,17 +201,17 @@ struct GroupLay {
   }
 };
 
-// mean and rstd of group blockIdx.x % groups of cloud blockIdx.x / groups, from the channels'
+// mean and rstd of a group of a cloud, from the channels'
 // means and squared deviations in the pieces of the cloud.  Sums over at most a few thousand
 // numbers, in double: their cost does not show.
 __global__ void __launch_bounds__(1024) norm_finish_kernel(const Norm a) {
   __shared__ double lds[3][16];
-  const int b = blockIdx.x / a.groups, g = blockIdx.x - b * a.groups;
+  const int id = a.first + (int)blockIdx.x, b = id / a.groups, g = id - b * a.groups;
   const int64_t s = cloud_begin(a, b), e = cloud_begin(a, b + 1);
   if (s >= e) {
     if (threadIdx.x == 0) {
-      a.mean[blockIdx.x] = 0.f;
-      a.rstd[blockIdx.x] = 0.f;
+      a.mean[id] = 0.f;
+      a.rstd[id] = 0.f;
     }
     return;
   }
@@ -244,8 +247,8 @@ __global__ void __launch_bounds__(1024) norm_finish_kernel(const Norm a) {
       for (int w = 0; w < (int)(blockDim.x >> 6); ++w) sums[i] += lds[i][w];
     }
     const double d = sums[1] / sums[0], var = sums[2] / sums[0] - d * d;
-    a.mean[blockIdx.x] = (float)(shift + d);
-    a.rstd[blockIdx.x] = (float)(1.0 / sqrt((var < 0 ? 0 : var) + (double)a.eps));
+    a.mean[id] = (float)(shift + d);
+    a.rstd[id] = (float)(1.0 / sqrt((var < 0 ? 0 : var) + (double)a.eps));
   }
 }
 
@@ -390,12 +393,12 @@ __global__ void __launch_bounds__(kThreads) norm_sums_kernel(const Norm a) {
   }
 }
 
-// Group blockIdx.x % groups of cloud blockIdx.x / groups: the pieces' sums added up, channel by
+// A group of a cloud: the pieces' sums added up, channel by
 // channel, and S1 / m, S2 / m of the group.
 __global__ void __launch_bounds__(1024) norm_reduce_kernel(const Norm a) {
   __shared__ float2 lds[1024];
   __shared__ float total[16];
-  const int b = blockIdx.x / a.groups, g = blockIdx.x - b * a.groups;
+  const int id = a.first + (int)blockIdx.x, b = id / a.groups, g = id - b * a.groups;
   const int64_t s = cloud_begin(a, b), e = cloud_begin(a, b + 1);
   const int k0 = (int)(s / a.rows), pieces = s < e ? (int)((e - 1) / a.rows) - k0 + 1 : 0;
   const float2 *p = a.partial + ((int64_t)k0 + b) * a.c + (int64_t)g * a.per;
@@ -438,7 +441,7 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const Norm a) {
   t2 = block_sum(t2, total);
   if (threadIdx.x == 0) {
     const float inv = s < e ? 1.f / ((float)(e - s) * (float)a.per) : 0.f;
-    a.group[blockIdx.x] = make_float2(t1 * inv, t2 * inv);
+    a.group[id] = make_float2(t1 * inv, t2 * inv);
   }
 }
 
@@ -541,14 +544,14 @@ struct FewLay {
 template <typename T>
 __global__ void __launch_bounds__(kFewThreads) norm_few_kernel(const Norm a) {
   __shared__ float lds[kFewThreads / 64];
-  const int b = blockIdx.x / a.groups, g = blockIdx.x - b * a.groups;
+  const int id = a.first + (int)blockIdx.x, b = id / a.groups, g = id - b * a.groups;
   const FewLay lay(a);
   const int64_t s = cloud_begin(a, b), e = cloud_begin(a, b + 1);
   const int64_t ch = (int64_t)g * a.per + lay.cx;
   const T *x = static_cast<const T *>(a.x) + ch;
   T *y = static_cast<T *>(a.out) + ch;
   if (s >= e) {
-    if (threadIdx.x == 0) a.mean[blockIdx.x] = a.rstd[blockIdx.x] = 0.f;
+    if (threadIdx.x == 0) a.mean[id] = a.rstd[id] = 0.f;
     return;
   }
   const float inv = 1.f / ((float)(e - s) * (float)a.per);
@@ -567,8 +570,8 @@ __global__ void __launch_bounds__(kFewThreads) norm_few_kernel(const Norm a) {
   }
   const float rstd = 1.f / sqrtf(block_sum(dev, lds) * inv + a.eps);
   if (threadIdx.x == 0) {
-    a.mean[blockIdx.x] = mean;
-    a.rstd[blockIdx.x] = rstd;
+    a.mean[id] = mean;
+    a.rstd[id] = rstd;
   }
   if (!lay.in) return;
   float w, bias;
@@ -586,12 +589,12 @@ template <typename T>
 __global__ void __launch_bounds__(kFewThreads) norm_few_backward_kernel(const Norm a) {
   __shared__ float2 lds[kFewThreads];
   __shared__ float total[kFewThreads / 64];
-  const int b = blockIdx.x / a.groups, g = blockIdx.x - b * a.groups;
+  const int id = a.first + (int)blockIdx.x, b = id / a.groups, g = id - b * a.groups;
   const FewLay lay(a);
   const int64_t s = cloud_begin(a, b), e = cloud_begin(a, b + 1);
   const int64_t ch = (int64_t)g * a.per + lay.cx;
   const T *x = static_cast<const T *>(a.x) + ch, *dy = static_cast<const T *>(a.dy) + ch;
-  const float mean = a.mean[blockIdx.x], rstd = a.rstd[blockIdx.x];
+  const float mean = a.mean[id], rstd = a.rstd[id];
   const int64_t r0 = lay.in ? s + lay.row : e;
   float w = 0.f, bias = 0.f, s1 = 0.f, s2 = 0.f;
   if (lay.in) channel_params<1>(a, ch, &w, &bias);
@@ -671,15 +674,27 @@ template <typename T> int width(const Norm &a) {
   else if (v == 4) SSC_NORM_LAUNCH(KERNEL, 4);                           \
   else SSC_NORM_LAUNCH(KERNEL, 1)
 
+// A workgroup to a cloud's group, in launches of at most 2^21 of them: a grid has fewer than 2^32
+// threads.
+constexpr int kGroupsMost = 1 << 21;
+template <typename K> void launch_groups(K kernel, Norm a, int threads, hipStream_t s) {
+  const int64_t all = (int64_t)a.clouds * a.groups;
+  for (int64_t at = 0; at < all; at += kGroupsMost) {
+    a.first = (int32_t)at;
+    const int64_t now = all - at < kGroupsMost ? all - at : kGroupsMost;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)now), dim3(threads), 0, s, a);
+  }
+}
+
 template <typename T> int forward(const Norm &a, hipStream_t s) {
   if (few(a)) {
-    hipLaunchKernelGGL(norm_few_kernel<T>, dim3(a.clouds * a.groups), dim3(kFewThreads), 0, s, a);
+    launch_groups(norm_few_kernel<T>, a, kFewThreads, s);
     SSC_LAUNCH_CHECK("group norm, forward");
     return SSC_OK;
   }
   const int v = width<T>(a);
   SSC_NORM_WIDTHS(norm_stats_kernel);
-  hipLaunchKernelGGL(norm_finish_kernel, dim3(a.clouds * a.groups), dim3(finish_threads(a)), 0, s, a);
+  launch_groups(norm_finish_kernel, a, finish_threads(a), s);
   SSC_NORM_WIDTHS(norm_apply_kernel);
   SSC_LAUNCH_CHECK("group norm, forward");
   return SSC_OK;
@@ -687,11 +702,11 @@ template <typename T> int forward(const Norm &a, hipStream_t s) {
 
 template <typename T> int backward(const Norm &a, hipStream_t s) {
   if (few(a)) {
-    hipLaunchKernelGGL(norm_few_backward_kernel<T>, dim3(a.clouds * a.groups), dim3(kFewThreads), 0, s, a);
+    launch_groups(norm_few_backward_kernel<T>, a, kFewThreads, s);
   } else {
     const int v = width<T>(a);
     SSC_NORM_WIDTHS(norm_sums_kernel);
-    hipLaunchKernelGGL(norm_reduce_kernel, dim3(a.clouds * a.groups), dim3(finish_threads(a)), 0, s, a);
+    launch_groups(norm_reduce_kernel, a, finish_threads(a), s);
     if (a.out) {
       SSC_NORM_WIDTHS(norm_dx_kernel);
     }
@@ -705,7 +720,7 @@ template <typename T> int backward(const Norm &a, hipStream_t s) {
 #undef SSC_NORM_LAUNCH
 
 size_t workspace(int64_t n, int32_t c, int32_t clouds, int32_t groups) {
-  if (n <= 0) return 256;
+  if (n <= 0 || c <= 0 || clouds <= 0 || groups <= 0) return 256;  // (the calls refuse all but no rows)
   const int64_t chunks = ceil_div(n, chunk_rows(n, c));
   return align_up((size_t)(chunks + clouds) * c * sizeof(float2)) +
          align_up((size_t)clouds * c * sizeof(float2)) +

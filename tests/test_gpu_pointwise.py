@@ -788,3 +788,52 @@ def test_pointwise_c_abi_refusals():
     assert lib.ssc_adamw_step(None, 0, 16, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1, None) == _ext.SSC_EINVAL
     assert lib.ssc_adamw_step(None, 0, 8, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1, None) == 0
     assert math.isfinite(float(x.sum()))
+
+
+@pytest.mark.parametrize("rows", [60, 6000])  # one launch, and passes over chunks
+def test_norm_of_squares_beyond_float(rows):
+    """Deviations whose squares pass float have an infinite variance: the bias is left."""
+    x, offsets, dy = norm_inputs([rows, rows], 16, torch.float32, 4)
+    want = group_norm(x, offsets, 2)
+    big = x.clone()
+    big[:rows, :8] *= 1e25
+    bias = normal((16,), 3)
+    got = group_norm(big.requires_grad_(), offsets, 2, None, bias)
+    assert torch.equal(got[:rows, :8], bias[:8].expand(rows, 8))
+    assert torch.equal(got[rows:] - bias, group_norm(x, offsets, 2, None, bias)[rows:] - bias)
+    assert want.isfinite().all()
+    dx, = torch.autograd.grad(got, big, dy)
+    assert not dx[:rows, :8].any() and dx.isfinite().all()
+
+
+@pytest.mark.parametrize("most", [1, 3])  # rows of a cloud: one launch, and passes over chunks
+def test_norm_of_more_groups_than_a_launch_has(most):
+    """40000 clouds of 64 groups are more workgroups than go into one grid."""
+    clouds, c, groups = 40000, 128, 64
+    size = torch.randint(0, most + 1, (clouds,), generator=torch.Generator().manual_seed(1))
+    if most == 1:
+        size[16000:39000] = 0  # (few rows)
+    ends = size.cumsum(0)
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), ends]).to(torch.int32).cuda()
+    n = int(ends[-1])
+    x, dy = normal((n, c), 2), normal((n, c), 3)
+    cloud = torch.repeat_interleave(torch.arange(clouds), size).cuda()
+
+    def mean_of(v):  # over the group of every element
+        s = torch.zeros(clouds, groups, dtype=torch.float64, device="cuda")
+        s.index_add_(0, cloud, v.view(n, groups, -1).sum(2))
+        return (s / (size.clamp(min=1).cuda()[:, None] * (c // groups)))[cloud].repeat_interleave(
+            c // groups, 1)
+
+    x64, g64 = x.double(), dy.double()
+    d = x64 - mean_of(x64)
+    rstd = 1 / torch.sqrt(mean_of(d * d) + 1e-2)
+    h = d * rstd
+    dx64 = rstd * (g64 - mean_of(g64) - h * mean_of(g64 * h))
+    x.requires_grad_()
+    y = group_norm(x, offsets, groups, eps=1e-2)
+    dx, = torch.autograd.grad(y, x, dy)
+    # sums of at most 6 values; |x|, |dy| below 6, rstd at most 10 and |h| below 3: a few units of
+    # float32 of the values at hand
+    within(y, h, rstd * 2.0 ** -19 + h.abs() * rstd * 2.0 ** -19, "y")
+    within(dx, dx64, (1 + rstd) ** 3 * 2.0 ** -16, "dx")
