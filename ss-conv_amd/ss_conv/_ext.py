@@ -1884,76 +1884,6 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def groupnorm_forward(x, offsets, groups, weight, bias, eps, act):
-    """y[n, c] and stats[2, clouds, groups] (mean, 1 / sqrt(var + eps)) of contiguous rows x[n, c]."""
-    n, c = x.shape
-    clouds = offsets.numel() - 1
-    y = torch.empty_like(x)
-    stats = torch.empty((2, clouds, groups), dtype=torch.float32, device=x.device)
-    ws = _workspace(_lib.ssc_groupnorm_workspace_bytes(n, c, clouds, groups), x.device)
-    mean = stats.data_ptr()
-    _check(_lib.ssc_groupnorm_fwd(
-        ELEM[x.dtype], _ptr(x), n, c, offsets.data_ptr(), clouds, groups,
-        _param_elem(x, weight, bias), _ptr(weight), _ptr(bias), eps, act, _ptr(y), mean,
-        mean + 4 * clouds * groups, ws.data_ptr(), ws.numel(), _raw_stream(x.get_device())))
-    return y, stats
-
-
-def groupnorm_backward(x, dy, offsets, groups, weight, bias, act, stats, want):
-    """dx, dweight, dbias (None where `want` says so) of contiguous rows x, dy [n, c], n >= 1."""
-    n, c = x.shape
-    clouds = offsets.numel() - 1
-    dx = torch.empty_like(x) if want[0] else None
-    dweight = torch.empty_like(weight) if want[1] else None
-    dbias = torch.empty_like(bias) if want[2] else None
-    ws = _workspace(_lib.ssc_groupnorm_workspace_bytes(n, c, clouds, groups), x.device)
-    mean = stats.data_ptr()
-    _check(_lib.ssc_groupnorm_bwd(
-        ELEM[x.dtype], x.data_ptr(), dy.data_ptr(), n, c, offsets.data_ptr(), clouds, groups,
-        _param_elem(x, weight, bias), _ptr(weight), _ptr(bias), act, mean,
-        mean + 4 * clouds * groups, _ptr(dx), _ptr(dweight), _ptr(dbias), ws.data_ptr(),
-        ws.numel(), _raw_stream(x.get_device())))
-    return dx, dweight, dbias
-
-
-def _param_elem(x, weight, bias):
-    """Element type of the parameters: both have the same, where there are any."""
-    return ELEM[(weight if weight is not None else bias if bias is not None else x).dtype]
-
-
-def gated_forward(x, w_gate, w_up, b_gate, b_up, act, keep):
-    """y[m, h] of contiguous rows x[m, k]; with `keep` also what the backward pass reads of both
-    projections (else None)."""
-    m, k = x.shape
-    h = w_gate.size(0)
-    y = x.new_empty((m, h))
-    elem = ELEM[x.dtype]
-    kept = _workspace(_lib.ssc_gated_kept_bytes(elem, m, h), x.device) if keep else None
-    ws = _workspace(_lib.ssc_gated_fwd_workspace_bytes(elem, m, k, h), x.device)
-    _check(_lib.ssc_gated_fwd(elem, _ptr(x), m, k, w_gate.data_ptr(), w_up.data_ptr(), h,
-                              _ptr(b_gate), _ptr(b_up), act, _ptr(y), _ptr(kept), ws.data_ptr(),
-                              ws.numel(), _raw_stream(x.get_device())))
-    return y, kept
-
-
-def gated_backward(x, w_gate, w_up, act, kept, dy, want):
-    """dx, dw_gate, dw_up, db_gate, db_up (None where `want` says so), m >= 1."""
-    m, k = x.shape
-    h = w_gate.size(0)
-    made = lambda like, yes: torch.empty_like(like) if yes else None  # noqa: E731
-    dx = made(x, want[0])
-    weights = want[1] or want[2]  # (one product gives both)
-    dw_gate, dw_up = made(w_gate, weights), made(w_up, weights)
-    db_gate, db_up = [x.new_empty(h) if w else None for w in want[3:5]]
-    elem = ELEM[x.dtype]
-    ws = _workspace(_lib.ssc_gated_bwd_workspace_bytes(elem, m, k, h), x.device)
-    _check(_lib.ssc_gated_bwd(elem, x.data_ptr(), m, k, w_gate.data_ptr(), w_up.data_ptr(), h, act,
-                              kept.data_ptr(), dy.data_ptr(), _ptr(dx), _ptr(dw_gate),
-                              _ptr(dw_up), _ptr(db_gate), _ptr(db_up), ws.data_ptr(), ws.numel(),
-                              _raw_stream(x.get_device())))
-    return dx, dw_gate if want[1] else None, dw_up if want[2] else None, db_gate, db_up
-
-
 def adamw_table(columns, count):
     """An array of ssc_adamw_tensor, whose fields are eight words each, from the columns param,
     grad, exp_avg, exp_avg_sq, scale, scale, numel, element type (None: zeros); addresses as

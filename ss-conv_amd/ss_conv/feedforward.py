@@ -14,30 +14,9 @@ import math
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
-from ss_conv import _ext
+from ss_conv import _pointwise
 from ss_conv import pointwise
-
-
-class _GatedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
-        y, kept = _ext.gated_forward(x, w_gate, w_up, b_gate, b_up, act, True)
-        ctx.save_for_backward(x, w_gate, w_up, kept)
-        ctx.act = act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, w_gate, w_up, kept = ctx.saved_tensors
-        want = ctx.needs_input_grad[:5]
-        if x.size(0) == 0:
-            shapes = (x, w_gate, w_up, w_gate[:, 0], w_gate[:, 0])
-            return tuple(torch.zeros_like(t) if w else None for t, w in zip(shapes, want)) + (None,)
-        return _ext.call_on(x, _ext.gated_backward, x, w_gate, w_up, ctx.act, kept,
-                            dy.contiguous(), want) + (None,)
 
 
 def _at_16_bytes(t):
@@ -51,13 +30,24 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     All tensors have one type (float32, float16 or bfloat16); biases [H] or None.
     activation: a name (None, "relu", "sigmoid", "tanh", "silu", "gelu"), the torch function or the
     torch.nn module of one.  Differentiable once in everything."""
+    act = pointwise.activation_code(activation)
+    y = _pointwise.gated_linear(x, w_gate, w_up, b_gate, b_up, act)
+    if y is None:  # something needs a look
+        y = _pointwise.gated_linear(*_laid_out(x, w_gate, w_up, b_gate, b_up), act)
+        pointwise.check_taken(y)
+        if x.dim() != 2:
+            y = y.view(x.shape[:-1] + y.shape[-1:])
+    return y
+
+
+def _laid_out(x, w_gate, w_up, b_gate, b_up):
+    """Checks gated_linear's arguments and lays them out as the kernels want them."""
     pointwise.check_rows("x", x)
     if x.dim() < 1:
         raise ValueError("x has no dimension")
     if not torch.is_tensor(w_gate) or w_gate.dim() != 2 or w_gate.size(0) < 1 or \
             w_gate.size(1) < 1:
         raise ValueError("w_gate is a matrix [hidden, width]")
-    act = pointwise.activation_code(activation)
     h, k = w_gate.shape
     if x.size(-1) != k:
         raise ValueError("x has {} columns, w_gate {}".format(x.size(-1), k))
@@ -66,15 +56,8 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
         pointwise.check_like(what, t, shape, (x.dtype,), x.device)
     if w_up is None:
         raise TypeError("w_up is missing")
-    rows = _at_16_bytes(x if x.dim() == 2 else x.reshape(-1, k))
-    w_gate, w_up = _at_16_bytes(w_gate), _at_16_bytes(w_up)
     b_gate, b_up = [None if t is None else t.contiguous() for t in (b_gate, b_up)]
-    args = (rows, w_gate, w_up, b_gate, b_up)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        y = _ext.call_on(x, _GatedLinear.apply, *args, act)
-    else:
-        y = _ext.call_on(x, _ext.gated_forward, *args, act, False)[0]
-    return y if x.dim() == 2 else y.view(x.shape[:-1] + (h,))
+    return [_at_16_bytes(t) for t in (x.reshape(-1, k), w_gate, w_up)] + [b_gate, b_up]
 
 
 class GatedLinear(nn.Module):

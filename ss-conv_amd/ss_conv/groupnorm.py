@@ -12,30 +12,9 @@ network equivariant; `ss_conv.batchnorm.BatchNorm` is the norm of fields of high
 """
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
-from ss_conv import _ext
+from ss_conv import _pointwise
 from ss_conv import pointwise
-
-
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, offsets, groups, eps, act):
-        y, stats = _ext.groupnorm_forward(x, offsets, groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, offsets, stats)
-        ctx.groups, ctx.act = groups, act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, offsets, stats = ctx.saved_tensors
-        want = ctx.needs_input_grad[:3]
-        if x.size(0) == 0:
-            made = [torch.zeros_like(t) if w else None for t, w in zip((x, weight, bias), want)]
-            return tuple(made) + (None,) * 4
-        return _ext.call_on(x, _ext.groupnorm_backward, x, dy.contiguous(), offsets, ctx.groups,
-                            weight, bias, ctx.act, stats, want) + (None,) * 4
 
 
 def group_norm(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
@@ -47,6 +26,17 @@ def group_norm(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activat
     activation: a name (None, "relu", "sigmoid", "tanh", "silu", "gelu"), the torch function or
     the torch.nn module of one.
     Differentiable once in x, weight and bias."""
+    act = pointwise.activation_code(activation)
+    y = _pointwise.group_norm(x, offsets, num_groups, weight, bias, eps, act)
+    if y is None:  # something needs a look
+        x, offsets, weight, bias = _laid_out(x, offsets, num_groups, weight, bias, eps)
+        y = _pointwise.group_norm(x, offsets, num_groups, weight, bias, eps, act)
+        pointwise.check_taken(y)
+    return y
+
+
+def _laid_out(x, offsets, num_groups, weight, bias, eps):
+    """Checks group_norm's arguments and lays them out as the kernels want them."""
     pointwise.check_rows("x", x)
     if x.dim() != 2:
         raise ValueError("x has {} dimensions, not 2".format(x.dim()))
@@ -55,7 +45,6 @@ def group_norm(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activat
         raise ValueError("{} channels cannot be cut into {} groups".format(c, num_groups))
     if not eps >= 0:
         raise ValueError("eps = {} is negative".format(eps))
-    act = pointwise.activation_code(activation)
     if not torch.is_tensor(offsets) or offsets.dim() != 1 or offsets.is_floating_point() or \
             offsets.is_complex() or offsets.dtype == torch.bool:
         raise TypeError("offsets is a vector of whole numbers")
@@ -68,17 +57,8 @@ def group_norm(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activat
     pointwise.check_like("bias", bias, (c,), kinds, x.device)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError("weight has type {}, bias {}".format(weight.dtype, bias.dtype))
-    offsets = offsets.to(torch.int32).contiguous()
-    x = x.contiguous()
-    grad = x.requires_grad
-    if weight is not None:
-        weight, grad = weight.contiguous(), grad or weight.requires_grad
-    if bias is not None:
-        bias, grad = bias.contiguous(), grad or bias.requires_grad
-    if grad and torch.is_grad_enabled():
-        return _ext.call_on(x, _GroupNorm.apply, x, weight, bias, offsets, num_groups, eps, act)
-    return _ext.call_on(x, _ext.groupnorm_forward, x, offsets, num_groups, weight, bias, eps,
-                        act)[0]
+    weight, bias = [None if t is None else t.contiguous() for t in (weight, bias)]
+    return x.contiguous(), offsets.to(torch.int32).contiguous(), weight, bias
 
 
 class GroupNorm(nn.Module):

@@ -13,12 +13,10 @@ Sparse gradients, gradients of another type than their parameter and tensors who
 fill their memory one after another are refused.  The number of the step is an argument of the
 launch: a step cannot be captured into a graph and replayed.
 """
-import itertools
-import operator
-
 import torch
 
 from ss_conv import _ext
+from ss_conv import _pointwise
 
 BLOCK = 256  # elements that share a scale
 
@@ -78,28 +76,8 @@ def _check_order(i, p, items):
                                             p.stride()))
 
 
-_dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
-
-
-def _usual(first, others, dtypes, sizes, blocks):
-    """Whether all tensors are contiguous and on one GPU, the i-th list of `others` is of dtypes[i]
-    and its tensors have `sizes` elements, or one for each block where blocks[i]: one pass over
-    the lists for each property, where checks tensor by tensor take several times as long."""
-    every = list(itertools.chain(first, *others))
-    try:
-        alike = all(map(torch.Tensor.is_contiguous, every))
-    except RuntimeError:  # (sparse tensors do not say)
-        return False
-    if not alike or not first[0].is_cuda or len(set(map(torch.Tensor.get_device, every))) != 1:
-        return False
-    scales = [_scales(n) for n in sizes] if any(blocks[:len(others)]) else None
-    return all(set(map(_dtype, x)) == {t} and list(map(torch.Tensor.numel, x)) ==
-               (scales if b else sizes) for x, t, b in zip(others, dtypes, blocks))
-
-
 _BITS8 = (torch.int8, torch.uint8, torch.float32, torch.float32)
 _BITS32 = (torch.float32, torch.float32)
-_BLOCKS = (False, False, True, True)  # which of them have one element for each block
 
 
 def _scales(n):
@@ -124,30 +102,30 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.99
             count, [len(x) for x in lists]))
     if count == 0:
         return
-    dtypes = _BITS8 if eight else _BITS32
-    dev = params[0].device
-    sizes, kinds = list(map(torch.Tensor.numel, params)), list(map(_dtype, params))
-    if not (set(kinds) <= _ext.ELEM.keys() and list(map(_dtype, grads)) == kinds and
-            list(map(_shape, grads)) == list(map(_shape, params)) and
-            _usual(list(params) + list(grads), lists[1:], dtypes, sizes, _BLOCKS)):
-        lists[0] = grads = list(grads)
-        for i, p in enumerate(params):
-            _check_param(i, p, grads[i])
-            if p.device != dev or grads[i].device != dev:
-                raise RuntimeError("parameter {} is on {}, its gradient on {}, the first on "
-                                   "{}".format(i, p.device, grads[i].device, dev))
-            n = p.numel()
-            _check_moments(i, n, dev, [x[i] for x in lists[1:]], dtypes,
-                           (n, n, _scales(n), _scales(n)))
-            _check_order(i, p, [x[i] for x in lists[1:3]])
-            grads[i] = _like(grads[i], p)
-    columns = [map(torch.Tensor.data_ptr, x) for x in [params] + lists]
-    if not eight:
-        columns += [None, None]
-    columns += [sizes, map(_ext.ELEM.__getitem__, kinds)]
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("an AdamW step cannot be captured into a graph: the number of the step "
                            "is an argument of its launch")
+    if _pointwise.adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales,
+                        step, lr, betas[0], betas[1], eps, weight_decay):
+        return
+    # something needs a look
+    dtypes = _BITS8 if eight else _BITS32
+    dev = params[0].device
+    lists[0] = grads = list(grads)
+    for i, p in enumerate(params):
+        _check_param(i, p, grads[i])
+        if p.device != dev or grads[i].device != dev:
+            raise RuntimeError("parameter {} is on {}, its gradient on {}, the first on "
+                               "{}".format(i, p.device, grads[i].device, dev))
+        n = p.numel()
+        _check_moments(i, n, dev, [x[i] for x in lists[1:]], dtypes,
+                       (n, n, _scales(n), _scales(n)))
+        _check_order(i, p, [x[i] for x in lists[1:3]])
+        grads[i] = _like(grads[i], p)
+    columns = [map(torch.Tensor.data_ptr, x) for x in [params] + lists]
+    if not eight:
+        columns += [None, None]
+    columns += [map(torch.Tensor.numel, params), [_ext.ELEM[p.dtype] for p in params]]
     _ext.call_on(params[0], _ext.adamw_step, columns, count, 8 if eight else 32, lr, betas[0],
                  betas[1], eps, weight_decay, step, _ext._raw_stream(dev.index))
     torch.autograd.graph.increment_version(params)
@@ -169,14 +147,16 @@ def state_values(exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, out=N
         out = tuple([torch.empty_like(t, dtype=torch.float32) for t in x]
                     for x in (exp_avgs, exp_avg_sqs))
     moments = [exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales]
-    sizes = list(map(torch.Tensor.numel, exp_avgs))
-    if not _usual(exp_avgs, moments + list(out), _BITS8 + _BITS32, sizes, _BLOCKS + _BLOCKS[:2]):
-        for i, n in enumerate(sizes):
-            _check_moments(i, n, dev, [x[i] for x in moments], _BITS8,
-                           (n, n, _scales(n), _scales(n)))
-            _check_moments(i, n, dev, (out[0][i], out[1][i]), _BITS32, (n, n))
-            # (a new tensor has the layout of the codes, a given one has to have it)
-            _check_order(i, exp_avgs[i], (exp_avg_sqs[i], out[0][i], out[1][i]))
+    if _pointwise.adamw_values(*out, *moments):
+        return tuple(out)
+    # something needs a look
+    sizes = [t.numel() for t in exp_avgs]
+    for i, n in enumerate(sizes):
+        _check_moments(i, n, dev, [x[i] for x in moments], _BITS8,
+                       (n, n, _scales(n), _scales(n)))
+        _check_moments(i, n, dev, (out[0][i], out[1][i]), _BITS32, (n, n))
+        # (a new tensor has the layout of the codes, a given one has to have it)
+        _check_order(i, exp_avgs[i], (exp_avg_sqs[i], out[0][i], out[1][i]))
     columns = [map(torch.Tensor.data_ptr, x) for x in list(out) + moments]
     columns += [sizes, None]
     _ext.call_on(exp_avgs[0], _ext.adamw_values, columns, count, _ext._raw_stream(dev.index))

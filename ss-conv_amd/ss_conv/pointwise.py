@@ -62,3 +62,9 @@ def check_like(what, t, shape, dtypes, device):
             what, t.dtype, " or ".join(str(d) for d in dict.fromkeys(dtypes))))
     if t.device != device:
         raise RuntimeError("{} is on {}, the rows are on {}".format(what, t.device, device))
+
+
+def check_taken(y):
+    """What the binding makes of arguments that have been checked and laid out."""
+    if y is None:
+        raise RuntimeError("tensors of this kind or size are not supported")

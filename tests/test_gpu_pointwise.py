@@ -837,3 +837,67 @@ def test_norm_of_more_groups_than_a_launch_has(most):
     # float32 of the values at hand
     within(y, h, rstd * 2.0 ** -19 + h.abs() * rstd * 2.0 ** -19, "y")
     within(dx, dx64, (1 + rstd) ** 3 * 2.0 ** -16, "dx")
+
+
+def pointwise_calls(dtype=torch.float32):
+    """(function, its differentiable arguments) of both layers, on a few rows."""
+    x, offsets, _ = norm_inputs([9, 4], 16, dtype, 2)
+    w, b = normal((16,), 3, dtype, 0.3, 1.0), normal((16,), 4, dtype)
+    wg, wu, bg = [normal(s, 5 + i, dtype, 0.3) for i, s in enumerate(((24, 16), (24, 16), (24,)))]
+    return [(lambda p, q, r: group_norm(p, offsets, 4, q, r, activation="silu"), (x, w, b)),
+            (lambda p, q, r, s: gated_linear(p, q, r, s), (x, wg, wu, bg))]
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_pointwise_autograd_rules(which):
+    call, args = pointwise_calls()[which]
+    leaves = [t.clone().requires_grad_() for t in args]
+    y = call(*leaves)
+    want = torch.autograd.grad(y.sum(), leaves, retain_graph=True)
+    # the same again, and for any of the inputs alone
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y.sum(), leaves), want))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y.sum(), leaves)
+    for i, t in enumerate(leaves):
+        assert torch.equal(torch.autograd.grad(call(*leaves).sum(), t)[0], want[i])
+    # once differentiable: what a gradient is made from is no constant
+    first = torch.autograd.grad(call(*leaves).sum(), leaves, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(first, want))
+    with pytest.raises(RuntimeError, match="differentiate"):
+        torch.autograd.grad(first[0].sum(), leaves)
+    # changed in place between forward and backward
+    z = [t.clone() for t in leaves]
+    y = call(*z)
+    with torch.no_grad():
+        z[0].add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    # no forward mode, which would lose its tangents without a word
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(args[0], torch.ones_like(args[0]))
+        with pytest.raises(RuntimeError):
+            call(dual, *args[1:])
+    with torch.inference_mode():
+        assert torch.equal(call(*args), call(*leaves))
+    with torch.no_grad():
+        assert not call(*leaves).requires_grad
+    assert not call(*args).requires_grad
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_pointwise_checkpoint_hooks_and_accumulation(which):
+    from torch.utils.checkpoint import checkpoint
+    call, args = pointwise_calls()[which]
+    leaves = [t.clone().requires_grad_() for t in args]
+    want = torch.autograd.grad(call(*leaves).sum(), leaves)
+    y = checkpoint(call, *leaves, use_reentrant=False)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y.sum(), leaves), want))
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.cpu()) or len(kept) - 1,
+                                                  lambda i: kept[i].cuda()):
+        y = call(*leaves)
+    assert len(kept) >= 4  # all that the backward pass reads goes through the hooks
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y.sum(), leaves), want))
+    for _ in range(2):
+        call(*leaves).sum().backward()
+    assert all(torch.equal(t.grad, 2 * g) for t, g in zip(leaves, want))
