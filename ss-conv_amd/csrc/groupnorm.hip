@@ -89,6 +89,46 @@ template <int V> struct Lay {
 
 constexpr int kUnroll = 4;  // rows of a thread whose loads are in flight together
 
+// Elements as they lie in memory: half the registers of their floats while they are on their way.
+template <typename T, int V> struct Raw {
+  typename Pack<T, V>::type v;
+  __device__ __forceinline__ void floats(float *out) const {
+    if constexpr (V == 1) {
+      out[0] = (float)v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = (float)v[i];
+    }
+  }
+};
+
+// The rows of a thread in s .. e - 1, kUnroll of them at a time.
+template <typename T, int V> struct Walk {
+  int64_t from, step;  // element of the next row; elements from one row of the thread to its next
+  int left;            // rows that are left of the thread's (a chunk's are fewer than 2^31)
+  __device__ __forceinline__ Walk(const Norm &a, const Lay<V> &lay, int64_t s, int64_t e)
+      : from((s + lay.row) * a.c), step((int64_t)lay.ty * a.c) {
+    const int rows = (int)(e - s) - lay.row;
+    left = rows > 0 ? (int)((uint32_t)(rows + lay.ty - 1) / (uint32_t)lay.ty) : 0;
+  }
+  __device__ __forceinline__ bool in(int u) const { return u < left; }
+  __device__ __forceinline__ int64_t at(int u) const { return from + u * step; }
+  __device__ __forceinline__ void next() {
+    from += kUnroll * step;
+    left -= kUnroll;
+  }
+  // ONCE: what is not read again need not push other lines out of the caches.
+  template <bool ONCE> __device__ __forceinline__ void load(const T *p, Raw<T, V> *out) const {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (in(u)) {
+        const auto *q = reinterpret_cast<const typename Pack<T, V>::type *>(p + at(u));
+        if constexpr (ONCE && V > 1) out[u].v = __builtin_nontemporal_load(q);
+        else out[u].v = *q;
+      }
+  }
+};
+
 // ---- statistics ---------------------------------------------------------------------------
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) norm_stats_kernel(const Norm a) {
@@ -107,32 +147,24 @@ __global__ void __launch_bounds__(kThreads) norm_stats_kernel(const Norm a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) first[i] = s1[i] = s2[i] = 0.f;
     if (lay.in && s + lay.row < e) {
-      int64_t r = s + lay.row;
-      load_floats<T, V>(x + r * a.c, first);
-      for (; r + (kUnroll - 1) * lay.ty < e; r += kUnroll * lay.ty) {
-        float v[kUnroll][V];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) load_floats<T, V>(x + (r + u * lay.ty) * a.c, v[u]);
+      load_floats<T, V>(x + (s + lay.row) * a.c, first);
+      Walk<T, V> walk(a, lay, s, e);
+      for (; walk.left > 0; walk.next()) {
+        Raw<T, V> v[kUnroll];
+        walk.template load<false>(x, v);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
+          if (walk.in(u)) {
+            float f[V];
+            v[u].floats(f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float d = v[u][i] - first[i];
-            s1[i] += d;
-            s2[i] += d * d;
+            for (int i = 0; i < V; ++i) {
+              const float d = f[i] - first[i];
+              s1[i] += d;
+              s2[i] += d * d;
+            }
+            count += 1.f;
           }
-        count += kUnroll;
-      }
-      for (; r < e; r += lay.ty) {
-        float v[V];
-        load_floats<T, V>(x + r * a.c, v);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = v[i] - first[i];
-          s1[i] += d;
-          s2[i] += d * d;
-        }
-        count += 1.f;
       }
     }
     const float inv = count > 0.f ? 1.f / count : 0.f;
@@ -253,24 +285,54 @@ __global__ void __launch_bounds__(1024) norm_finish_kernel(const Norm a) {
 }
 
 // ---- y --------------------------------------------------------------------------------------
-// What the channels of a thread need of cloud b.
-template <int V>
-__device__ __forceinline__ void channel_consts(const Norm &a, int b, int64_t ch, float *mean,
-                                               float *rstd) {
+// Elements of the groups of cloud b that the channels ch .. of a thread lie in: one load where they
+// are one group's.
+template <int V, typename E>
+__device__ __forceinline__ void of_groups(const Norm &a, const E *p, int b, int64_t ch, E *out) {
+  const uint32_t per = (uint32_t)a.per, g0 = (uint32_t)ch / per;
+  p += (int64_t)b * a.groups + g0;
+  if (per % V == 0) {
+    const E e = *p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = e;
+    return;
+  }
+  uint32_t at = (uint32_t)ch - g0 * per, g = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int64_t g = (int64_t)b * a.groups + (ch + i) / a.per;
-    mean[i] = a.mean[g];
-    rstd[i] = a.rstd[g];
+    out[i] = p[g];
+    if (++at == per) {
+      at = 0;
+      ++g;
+    }
+  }
+}
+// V neighbouring elements of a parameter, `none` without one.
+template <int V>
+__device__ __forceinline__ void of_channels(const void *p, int64_t ch, int type, float none, float *out) {
+  const size_t bytes = type == SSC_F32 ? 4 : 2;
+  if (p == nullptr) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = none;
+  } else if (V > 1 && (reinterpret_cast<uintptr_t>(p) & ((V * bytes < 16 ? V * bytes : 16) - 1)) == 0) {
+    // (ch is a multiple of V)
+    if (type == SSC_F32) {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) load_floats<float, V < 4 ? V : 4>(static_cast<const float *>(p) + ch + i, out + i);
+    } else if (type == SSC_F16) {
+      load_floats<f16, V>(static_cast<const f16 *>(p) + ch, out);
+    } else {
+      load_floats<bf16, V>(static_cast<const bf16 *>(p) + ch, out);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = load_any(p, ch + i, type);
   }
 }
 template <int V>
 __device__ __forceinline__ void channel_params(const Norm &a, int64_t ch, float *w, float *bias) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    w[i] = a.weight ? load_any(a.weight, ch + i, a.wtype) : 1.f;
-    bias[i] = a.bias ? load_any(a.bias, ch + i, a.wtype) : 0.f;
-  }
+  of_channels<V>(a.weight, ch, a.wtype, 1.f, w);
+  of_channels<V>(a.bias, ch, a.wtype, 0.f, bias);
 }
 
 template <typename T, int V>
@@ -289,21 +351,23 @@ __global__ void __launch_bounds__(kThreads) norm_apply_kernel(const Norm a) {
     const int64_t s = cb > r0 ? cb : r0, e = ce < r1 ? ce : r1;
     if (s >= e) continue;
     float mean[V], rstd[V];
-    channel_consts<V>(a, b, lay.ch, mean, rstd);
+    of_groups<V>(a, a.mean, b, lay.ch, mean);
+    of_groups<V>(a, a.rstd, b, lay.ch, rstd);
 #pragma unroll
     for (int i = 0; i < V; ++i) rstd[i] *= w[i];
-    for (int64_t r = s + lay.row; r < e; r += lay.ty * kUnroll) {
-      float v[kUnroll][V], z[V];
+    Walk<T, V> walk(a, lay, s, e);
+    for (; walk.left > 0; walk.next()) {
+      Raw<T, V> v[kUnroll];
+      walk.template load<true>(x, v);
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
-        if (r + u * lay.ty < e) load_floats_once<T, V>(x + (r + u * lay.ty) * a.c, v[u]);
+        if (walk.in(u)) {
+          float z[V], f[V];
+          v[u].floats(z);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (r + u * lay.ty < e) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) z[i] = (v[u][i] - mean[i]) * rstd[i] + bias[i];
-          activate<V>(a.act, z, v[u]);
-          store_floats_once<T, V>(y + (r + u * lay.ty) * a.c, v[u]);
+          for (int i = 0; i < V; ++i) z[i] = (z[i] - mean[i]) * rstd[i] + bias[i];
+          activate<V>(a.act, z, f);
+          store_floats_once<T, V>(y + walk.at(u), f);
         }
     }
   }
@@ -346,20 +410,20 @@ __global__ void __launch_bounds__(kThreads) norm_sums_kernel(const Norm a) {
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
     if (lay.in) {
       float mean[V], rstd[V];
-      channel_consts<V>(a, b, lay.ch, mean, rstd);
-      for (int64_t r = s + lay.row; r < e; r += lay.ty * kUnroll) {
-        float v[kUnroll][V], g[kUnroll][V];
+      of_groups<V>(a, a.mean, b, lay.ch, mean);
+      of_groups<V>(a, a.rstd, b, lay.ch, rstd);
+      Walk<T, V> walk(a, lay, s, e);
+      for (; walk.left > 0; walk.next()) {
+        Raw<T, V> v[kUnroll], g[kUnroll];
+        walk.template load<false>(x, v);
+        walk.template load<false>(dy, g);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-          if (r + u * lay.ty < e) {
-            load_floats<T, V>(x + (r + u * lay.ty) * a.c, v[u]);
-            load_floats<T, V>(dy + (r + u * lay.ty) * a.c, g[u]);
-          }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          if (r + u * lay.ty < e) {
-            float h[V], dz[V];
-            row_terms<V>(a.act, v[u], g[u], mean, rstd, w, bias, h, dz);
+          if (walk.in(u)) {
+            float xv[V], gv[V], h[V], dz[V];
+            v[u].floats(xv);
+            g[u].floats(gv);
+            row_terms<V>(a.act, xv, gv, mean, rstd, w, bias, h, dz);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
               s1[i] += dz[i];
@@ -489,30 +553,26 @@ __global__ void __launch_bounds__(kThreads) norm_dx_kernel(const Norm a) {
     if (cb >= r1) break;
     const int64_t s = cb > r0 ? cb : r0, e = ce < r1 ? ce : r1;
     if (s >= e) continue;
-    float mean[V], rstd[V], m1[V], m2[V];
-    channel_consts<V>(a, b, lay.ch, mean, rstd);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float2 v = a.group[(int64_t)b * a.groups + (lay.ch + i) / a.per];
-      m1[i] = v.x;
-      m2[i] = v.y;
-    }
-    for (int64_t r = s + lay.row; r < e; r += lay.ty * kUnroll) {
-      float v[kUnroll][V], g[kUnroll][V];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (r + u * lay.ty < e) {
-          load_floats_once<T, V>(x + (r + u * lay.ty) * a.c, v[u]);
-          load_floats_once<T, V>(dy + (r + u * lay.ty) * a.c, g[u]);
-        }
+    float mean[V], rstd[V];
+    float2 m[V];
+    of_groups<V>(a, a.mean, b, lay.ch, mean);
+    of_groups<V>(a, a.rstd, b, lay.ch, rstd);
+    of_groups<V>(a, a.group, b, lay.ch, m);
+    Walk<T, V> walk(a, lay, s, e);
+    for (; walk.left > 0; walk.next()) {
+      Raw<T, V> v[kUnroll], g[kUnroll];
+      walk.template load<true>(x, v);
+      walk.template load<true>(dy, g);
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
-        if (r + u * lay.ty < e) {
-          float h[V], dz[V];
-          row_terms<V>(a.act, v[u], g[u], mean, rstd, w, bias, h, dz);
+        if (walk.in(u)) {
+          float xv[V], gv[V], h[V], dz[V];
+          v[u].floats(xv);
+          g[u].floats(gv);
+          row_terms<V>(a.act, xv, gv, mean, rstd, w, bias, h, dz);
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[u][i] = rstd[i] * (w[i] * dz[i] - (m1[i] + h[i] * m2[i]));
-          store_floats_once<T, V>(dx + (r + u * lay.ty) * a.c, v[u]);
+          for (int i = 0; i < V; ++i) xv[i] = rstd[i] * (w[i] * dz[i] - (m[i].x + h[i] * m[i].y));
+          store_floats_once<T, V>(dx + walk.at(u), xv);
         }
     }
   }
