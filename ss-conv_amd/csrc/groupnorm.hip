@@ -16,8 +16,9 @@
 // The second pass takes the chunks from the last one on, reads its inputs for the last time and
 // writes past the caches: what the first pass read last is then still in the 256 MB of the last
 // cache level.  600153 x 128 floats, forward and backward: 519 us with both passes in order, 492 with
-// the second one reversed, 436 with writes and last reads past the caches as well (an x of 307 MB
-// moves 2.46 GB, 476 us at the 5.16 TB/s of a large copy, if no cache helps).
+// the second one reversed, 436 with writes and last reads past the caches as well, 428 with half as
+// many chunks (an x of 307 MB moves 2.46 GB, 476 us at the 5.16 TB/s of a large copy, if no cache
+// helps).
 //
 // The variance comes from deviations, not from E[x^2] - mean^2: a thread sums x - x0 and
 // (x - x0)^2 with its own first value x0 of the channel, which leaves numbers of the spread's
@@ -30,7 +31,10 @@ namespace ssc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunksMost = 2048;  // chunks of rows: eight workgroups for each of 256 CUs
+// Chunks of rows: four workgroups for each of 256 CUs.  More of them pay for finding their cloud and for
+// adding up too often: forward and backward with 2048, 1024 and 512 chunks 50001 x 200 float16 76, 67 and
+// 70 us, 100000 x 64 bfloat16 69, 61 and 57, 600153 x 128 floats 437, 432 and 451.
+constexpr int kChunksMost = 1024;
 
 struct Norm {
   const void *x, *dy;
@@ -44,6 +48,7 @@ struct Norm {
   void *dweight, *dbias;     // [c] or NULL
   int64_t n;
   int32_t c, clouds, groups, per, wtype, act, rows;  // rows: of a chunk
+  int32_t chunks;
   int32_t first;             // a launch with a workgroup to a cloud's group: the first one's number
   float eps;
 };
@@ -87,7 +92,8 @@ template <int V> struct Lay {
   }
 };
 
-constexpr int kUnroll = 4;  // rows of a thread whose loads are in flight together
+// Rows of a thread whose loads are in flight together (four: 3 % slower, by their registers).
+constexpr int kUnroll = 2;
 
 // Elements as they lie in memory: half the registers of their floats while they are on their way.
 template <typename T, int V> struct Raw {
@@ -537,8 +543,15 @@ __global__ void __launch_bounds__(kThreads) norm_params_kernel(const Norm a) {
   param_grads(a, blockIdx.x);
 }
 
+// The parameters' gradients need no launch of their own: the workgroups in front of the chunks'
+// make them (50001 x 200 float16, forward and backward: 2 us of 67 less).
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) norm_dx_kernel(const Norm a) {
+  const int before = (int)gridDim.x - a.chunks;
+  if ((int)blockIdx.x < before) {
+    if (blockIdx.y == 0) param_grads(a, blockIdx.x);
+    return;
+  }
   const Lay<V> lay(a);
   if (!lay.in) return;
   const int64_t r0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * a.rows;
@@ -582,13 +595,13 @@ __global__ void __launch_bounds__(kThreads) norm_dx_kernel(const Norm a) {
 // A workgroup to a cloud's group, all passes in one launch: the rows of a group lie in the caches
 // after the first pass.  Threads: `per` channels side by side, kFewThreads / per rows at a time.
 constexpr int kFewThreads = 512;
-// The form pays up to some 8000 values of a group: 2100 rows in 2 clouds, 4 channels in a group
-// (4200 values), forward and backward 7 and 12 us against 15 and 17 of the passes over chunks; 1024
-// rows of 8 channels 10 and 20 against 14 and 17; 1024 rows of 16 channels 13 and 20 against 13 and
-// 15.  How many rows a cloud has is not known here: the mean is taken, and a limit for all rows, so
+// The form pays up to some 8192 values of a group: 2100 rows in 2 clouds, 4 channels in a group
+// (4200 values), forward and backward 8 and 11 us against 15 and 17 of the passes over chunks; 1024
+// rows of 8 channels 9 and 13 against 12 and 14; 1024 rows of 16 channels 14 and 20 against 12 and
+// 14.  How many rows a cloud has is not known here: the mean is taken, and a limit for all rows, so
 // that a batch whose rows are nearly all one cloud's stays near (32768 values of one group: 23 and
-// 35 us against 13 and 15).
-constexpr int64_t kFewMean = 6144, kFewMost = 32768;
+// 34 us against 12 and 14).
+constexpr int64_t kFewMean = 8192, kFewMost = 32768;
 
 struct FewLay {
   int ty, row, cx;
@@ -705,15 +718,15 @@ bool same_alignment(const void *a, const void *b, const void *c, size_t to) {
            reinterpret_cast<uintptr_t>(c)) & (to - 1)) == 0;
 }
 
-dim3 chunk_grid(const Norm &a, int v) {
+dim3 chunk_grid(const Norm &a, int v, int before) {
   const int cv = a.c / v;
   const int tx = cv < kThreads ? cv : kThreads;
-  return dim3((uint32_t)ceil_div(a.n, a.rows), (uint32_t)ceil_div(cv, tx));
+  return dim3((uint32_t)(a.chunks + before), (uint32_t)ceil_div(cv, tx));
 }
 
 // Threads of a workgroup that adds up the pieces of one group.
 int finish_threads(const Norm &a) {
-  const int64_t items = (ceil_div(a.n, a.rows) / a.clouds + 1) * a.per;
+  const int64_t items = (int64_t)(a.chunks / a.clouds + 1) * a.per;
   return items > 2048 ? 1024 : items > 256 ? 256 : 64;
 }
 
@@ -727,12 +740,13 @@ template <typename T> int width(const Norm &a) {
   if (a.c % V == 0 && same_alignment(a.x, a.dy, a.out, 16)) return V;
   return V == 8 && a.c % 4 == 0 && same_alignment(a.x, a.dy, a.out, 8) ? 4 : 1;
 }
-#define SSC_NORM_LAUNCH(KERNEL, V) \
-  hipLaunchKernelGGL((KERNEL<T, V>), chunk_grid(a, V), dim3(kThreads), 0, s, a)
-#define SSC_NORM_WIDTHS(KERNEL)                                         \
-  if (v == 16 / (int)sizeof(T)) SSC_NORM_LAUNCH(KERNEL, 16 / sizeof(T)); \
-  else if (v == 4) SSC_NORM_LAUNCH(KERNEL, 4);                           \
-  else SSC_NORM_LAUNCH(KERNEL, 1)
+// (BEFORE: workgroups in front of the chunks')
+#define SSC_NORM_LAUNCH(KERNEL, V, BEFORE) \
+  hipLaunchKernelGGL((KERNEL<T, V>), chunk_grid(a, V, BEFORE), dim3(kThreads), 0, s, a)
+#define SSC_NORM_WIDTHS(KERNEL, BEFORE)                                         \
+  if (v == 16 / (int)sizeof(T)) SSC_NORM_LAUNCH(KERNEL, 16 / sizeof(T), BEFORE); \
+  else if (v == 4) SSC_NORM_LAUNCH(KERNEL, 4, BEFORE);                           \
+  else SSC_NORM_LAUNCH(KERNEL, 1, BEFORE)
 
 // A workgroup to a cloud's group, in launches of at most 2^21 of them: a grid has fewer than 2^32
 // threads.
@@ -753,26 +767,27 @@ template <typename T> int forward(const Norm &a, hipStream_t s) {
     return SSC_OK;
   }
   const int v = width<T>(a);
-  SSC_NORM_WIDTHS(norm_stats_kernel);
+  SSC_NORM_WIDTHS(norm_stats_kernel, 0);
   launch_groups(norm_finish_kernel, a, finish_threads(a), s);
-  SSC_NORM_WIDTHS(norm_apply_kernel);
+  SSC_NORM_WIDTHS(norm_apply_kernel, 0);
   SSC_LAUNCH_CHECK("group norm, forward");
   return SSC_OK;
 }
 
 template <typename T> int backward(const Norm &a, hipStream_t s) {
+  int params = a.dweight || a.dbias ? (int)ceil_div(a.c, 16) : 0;  // workgroups that make their gradients
   if (few(a)) {
     launch_groups(norm_few_backward_kernel<T>, a, kFewThreads, s);
   } else {
     const int v = width<T>(a);
-    SSC_NORM_WIDTHS(norm_sums_kernel);
+    SSC_NORM_WIDTHS(norm_sums_kernel, 0);
     launch_groups(norm_reduce_kernel, a, finish_threads(a), s);
     if (a.out) {
-      SSC_NORM_WIDTHS(norm_dx_kernel);
+      SSC_NORM_WIDTHS(norm_dx_kernel, params);
+      params = 0;
     }
   }
-  if (a.dweight || a.dbias)
-    hipLaunchKernelGGL(norm_params_kernel, dim3((uint32_t)ceil_div(a.c, 16)), dim3(kThreads), 0, s, a);
+  if (params > 0) hipLaunchKernelGGL(norm_params_kernel, dim3(params), dim3(kThreads), 0, s, a);
   SSC_LAUNCH_CHECK("group norm, backward");
   return SSC_OK;
 }
@@ -811,8 +826,9 @@ Norm carve(int64_t n, int32_t c, int32_t clouds, int32_t groups, void *ws) {
   a.groups = groups;
   a.per = c / groups;
   a.rows = (int32_t)chunk_rows(n, c);
+  a.chunks = (int32_t)ceil_div(n, a.rows);
   Carver w(ws);
-  a.partial = w.take<float2>((size_t)(ceil_div(n, a.rows) + clouds) * c);
+  a.partial = w.take<float2>((size_t)(a.chunks + clouds) * c);
   a.sums = w.take<float2>((size_t)clouds * c);
   a.group = w.take<float2>((size_t)clouds * groups);
   return a;
