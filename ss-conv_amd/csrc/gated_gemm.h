@@ -209,20 +209,26 @@ template <int R, int BK, int W> struct Side<R, BK, W, true> {
 
 // The same for floats, 8 of them to a thread at a time: fetched into registers one step before they
 // are cut into parts and stored to LDS, so that the way from memory is covered by a whole step.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void cut_into_parts(const f32x4 (&v)[2], char *to, int stride) {
-  bf16x8 p[3];
+  uint32_t p[3][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = v[i / 4][i % 4];
+  for (int i = 0; i < 4; ++i) {  // (pairs: one instruction rounds two floats)
+    const f32x2 x = {v[i / 2][i % 2 * 2], v[i / 2][i % 2 * 2 + 1]};
     // the first part is cut off, which no finite number overflows at, the others are rounded
-    const float a0 = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), r = x - a0;
-    const bf16 a1 = (bf16)r;
-    p[0][i] = __builtin_bit_cast(bf16, (unsigned short)(__float_as_uint(x) >> 16));
-    p[1][i] = a1;
-    p[2][i] = (bf16)(r - (float)a1);
+    f32x2 r;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) r[e] = x[e] - __uint_as_float(__float_as_uint(x[e]) & 0xFFFF0000u);
+    p[0][i] = __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x07060302);
+    p[1][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+    r[0] -= __uint_as_float(p[1][i] << 16);
+    r[1] -= __uint_as_float(p[1][i] & 0xFFFF0000u);
+    p[2][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
   }
 #pragma unroll
-  for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8 *>(to + k * stride) = p[k];
+  for (int k = 0; k < 3; ++k)
+    *reinterpret_cast<uint4 *>(to + k * stride) = make_uint4(p[k][0], p[k][1], p[k][2], p[k][3]);
 }
 
 template <int R, int BK, int W, bool TR> struct FloatSide : Side<R, BK, W, false> {
@@ -250,18 +256,21 @@ template <int R, int BK, int W, bool TR> struct FloatSide : Side<R, BK, W, false
           rows > 0 ? (int)(rows * o.ld * 4) : 0, 0x00020000);
     }
   }
-  __device__ __forceinline__ void fetch(const Operand &, int k0, int k_end) {
+  __device__ __forceinline__ void fetch(const Operand &, int k0) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        v[i][h] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs[i], off + k0 * 4 + h * 16, 0, 0));
+  }
+  // Zeros for what lies behind the end: behind a row's end lies the next row.
+  __device__ __forceinline__ void end(int k0, int k_end) {
     const int left = k_end - k0 - kc;  // values of this thread that exist
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v[i][h] = __builtin_bit_cast(
-            f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs[i], off + k0 * 4 + h * 16, 0, 0));
-        // (behind a row's end lies the next row)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][h][e] = h * 4 + e < left ? v[i][h][e] : 0.f;
-      }
+      for (int e = 0; e < 8; ++e) v[i][e / 4][e % 4] = e < left ? v[i][e / 4][e % 4] : 0.f;
   }
   __device__ __forceinline__ void store(char *tile, int stride) const {
 #pragma unroll
@@ -299,7 +308,7 @@ template <int R, int BK, int W> struct FloatSide<R, BK, W, true> : Side<R, BK, W
     }
   }
   // (behind the last column lies the next row: columns of results that are not stored)
-  __device__ __forceinline__ void fetch(const Operand &o, int, int) {
+  __device__ __forceinline__ void fetch(const Operand &o, int) {
     const int there = left < BK ? (int)left : BK;
     const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)cur, 0,
                                                       there > 0 ? (there - 1) * row + rest : 0, 0x00020000);
@@ -313,6 +322,7 @@ template <int R, int BK, int W> struct FloatSide<R, BK, W, true> : Side<R, BK, W
     cur = turn ? next : cur + (int64_t)BK * row;
     left = turn ? (int64_t)o.deep : left - BK;
   }
+  __device__ __forceinline__ void end(int, int) {}  // (the resource ends there)
   __device__ __forceinline__ void store(char *tile, int stride) const {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) cut_into_parts(v[i], tile + to[i], stride);
@@ -537,19 +547,27 @@ __global__ void __launch_bounds__(C::kThreads) gemm_kernel(const GemmArgs g) {
     // Two stages in LDS: while one is multiplied the next step's floats are cut into the other one,
     // and those of the step behind it are under way.
     auto fetch = [&](int k0) {
-      sa.fetch(g.a, k0, k_end);
-      sb.fetch(g.b, k0, k_end);
+      sa.fetch(g.a, k0);
+      sb.fetch(g.b, k0);
+    };
+    // (a branch of its own, so that all but the last step is one run of instructions)
+    auto end = [&](int k0) {
+      if (k0 + C::BK <= k_end) return;
+      sa.end(k0, k_end);
+      sb.end(k0, k_end);
     };
     auto store = [&](int s) {
       sa.store(lds + s * C::kStage, C::kABytes);
       sb.store(lds + s * C::kStage + 3 * C::kABytes, C::kBBytes);
     };
     fetch(k_begin);
+    end(k_begin);
     store(0);
     fetch(k_begin + C::BK);
     int s = 0;
     for (int k0 = k_begin; k0 < k_end; k0 += C::BK, s ^= 1) {
       __syncthreads();
+      end(k0 + C::BK);
       Blocks<C> x;
       read_blocks<C, SA, SB>(lds + s * C::kStage, 0, wm, wn, x);
       store(s ^ 1);  // (behind the last step these are zeros)
