@@ -332,7 +332,7 @@ template <typename C> int slices_of(const Shape &s) {
 // storing takes longer than multiplying then, and a CU holds only one large tile.  25600 rows ->
 // 1024, kept, bfloat16, large against middle tiles: k = 128 73 and 66 us, 256 82 and 81, 512 105 and
 // 110; 25437 -> 808, k = 128, float16 118 and 61.  Floats, large against small: 25600 -> 1024 kept,
-// k = 64 133 and 130, 128 154 and 162; 4096 -> 4096 kept, k = 64 86 and 69, 256 139 and 157.
+// k = 64 133 and 135, 128 156 and 164; 4096 -> 4096 kept, k = 64 101 and 68, 256 143 and 145.
 template <typename T> int forward_size(const Shape &s, bool kept) {
   const bool stores = kept && s.k <= (sizeof(T) == 4 ? 64 : 384);
   if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) >= kCUs && !stores) return 2;
@@ -342,8 +342,8 @@ template <typename T> int forward_size(const Shape &s, bool kept) {
 // of them; the tile's reuse counts for more the longer the product takes (times with the pass that
 // makes da and db).  bfloat16, large, middle, small: 25600 x 2048 (k) x 2048 293, 363, 377 us; 25600 x
 // 1024 (k) x 2048 207, 203, 283; 16384 x 512 (k) x 2048 101, 74, 78; 1024 x 2048 (k) x 2048 49, 45, 38.
-// Floats, large and small: 57304 x 1024 (k) x 128 110 and 138; 16384 x 512 (k) x 256 60 and 53; 1024 x
-// 2048 (k) x 1024 48 and 46; 300 x 8192 (k) x 2048 107 and 92.
+// Floats, large and small: 57304 x 1024 (k) x 128 203 and 226; 16384 x 512 (k) x 256 60 and 53; 1024 x
+// 2048 (k) x 1024 47 and 46; 300 x 8192 (k) x 2048 99 and 92.
 template <typename T> int product_size(const Shape &s) {
   const double work = (double)s.m * s.n * s.k;
   if (tiles_of<typename Tiles<T>::Large>(s.m, s.n) >= kCUs * 3 / 4) return 2;
@@ -405,13 +405,13 @@ struct Problem {
 };
 
 // Whether the few-rows kernel is taken: for 16 bits up to 64 rows, or a workgroup to a CU; for
-// floats, which it takes as they are where tiles want them in parts, up to 896 workgroups.  It
+// floats, which it takes as they are where tiles want them in parts, up to two to a CU.  It
 // against tiles, us: bfloat16, 1024 -> 1024, 256 rows 9.5 and 10.5, 384 rows 14.8 and 10.7; 2048 ->
-// 4096, 64 rows 16 and 22, 96 rows 24 and 22; floats, 1000 -> 2728, 256 rows 47 and 57, 512 rows 89
-// and 84; 2048 -> 4096, 192 rows 90 and 107, 256 rows 122 and 113; 128 -> 512, 512 rows 5.6 and 11.
+// 4096, 64 rows 16 and 22, 96 rows 24 and 22; floats, 2048 -> 4096, 128 rows 56 and 65, 192 rows 85
+// and 68; 1000 -> 2728, 256 rows 46 and 38; 128 -> 512, 512 rows 5.6 and 8.3.
 template <typename T> bool takes_few(const Problem &p) {
   const int64_t groups = ceil_div(p.h, 16) * ceil_div(p.m, 64);
-  return sizeof(T) == 4 ? groups <= 896 : p.m <= 64 || groups <= kCUs;
+  return sizeof(T) == 4 ? groups <= 2 * kCUs : p.m <= 64 || groups <= kCUs;
 }
 
 // x and the weights as the matrix kernel reads them: as they are, or laid out anew in ws.
