@@ -342,7 +342,10 @@ bool adamw(py::handle params, py::handle grads, py::handle m, py::handle v, py::
   const c10::DeviceGuard guard(first.device());
   check(ssc_adamw_step(table.data(), (int32_t)p.count, eight ? 8 : 32, lr, beta1, beta2, eps, weight_decay, step,
                        stream_of(first)));
-  for (Py_ssize_t i = 0; i < p.count; ++i) THPVariable_Unpack(p.items[i]).unsafeGetTensorImpl()->bump_version();
+  for (Py_ssize_t i = 0; i < p.count; ++i) {
+    const Tensor &t = THPVariable_Unpack(p.items[i]);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
   return true;
 }
 

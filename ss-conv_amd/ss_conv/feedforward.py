@@ -15,7 +15,6 @@ import math
 import torch
 import torch.nn as nn
 
-from ss_conv import _pointwise
 from ss_conv import pointwise
 
 
@@ -31,9 +30,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     activation: a name (None, "relu", "sigmoid", "tanh", "silu", "gelu"), the torch function or the
     torch.nn module of one.  Differentiable once in everything."""
     act = pointwise.activation_code(activation)
-    y = _pointwise.gated_linear(x, w_gate, w_up, b_gate, b_up, act)
+    y = pointwise.binding.gated_linear(x, w_gate, w_up, b_gate, b_up, act)
     if y is None:  # something needs a look
-        y = _pointwise.gated_linear(*_laid_out(x, w_gate, w_up, b_gate, b_up), act)
+        y = pointwise.binding.gated_linear(*_laid_out(x, w_gate, w_up, b_gate, b_up), act)
         pointwise.check_taken(y)
         if x.dim() != 2:
             y = y.view(x.shape[:-1] + y.shape[-1:])

@@ -13,7 +13,6 @@ network equivariant; `ss_conv.batchnorm.BatchNorm` is the norm of fields of high
 import torch
 import torch.nn as nn
 
-from ss_conv import _pointwise
 from ss_conv import pointwise
 
 
@@ -27,10 +26,10 @@ def group_norm(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activat
     the torch.nn module of one.
     Differentiable once in x, weight and bias."""
     act = pointwise.activation_code(activation)
-    y = _pointwise.group_norm(x, offsets, num_groups, weight, bias, eps, act)
+    y = pointwise.binding.group_norm(x, offsets, num_groups, weight, bias, eps, act)
     if y is None:  # something needs a look
         x, offsets, weight, bias = _laid_out(x, offsets, num_groups, weight, bias, eps)
-        y = _pointwise.group_norm(x, offsets, num_groups, weight, bias, eps, act)
+        y = pointwise.binding.group_norm(x, offsets, num_groups, weight, bias, eps, act)
         pointwise.check_taken(y)
     return y
 

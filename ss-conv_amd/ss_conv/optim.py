@@ -16,7 +16,7 @@ launch: a step cannot be captured into a graph and replayed.
 import torch
 
 from ss_conv import _ext
-from ss_conv import _pointwise
+from ss_conv import pointwise
 
 BLOCK = 256  # elements that share a scale
 
@@ -105,8 +105,9 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.99
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("an AdamW step cannot be captured into a graph: the number of the step "
                            "is an argument of its launch")
-    if _pointwise.adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales,
-                        step, lr, betas[0], betas[1], eps, weight_decay):
+    if pointwise.binding.adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales,
+                               exp_avg_sq_scales, step, lr, betas[0], betas[1], eps,
+                               weight_decay):
         return
     # something needs a look
     dtypes = _BITS8 if eight else _BITS32
@@ -147,7 +148,7 @@ def state_values(exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, out=N
         out = tuple([torch.empty_like(t, dtype=torch.float32) for t in x]
                     for x in (exp_avgs, exp_avg_sqs))
     moments = [exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales]
-    if _pointwise.adamw_values(*out, *moments):
+    if pointwise.binding.adamw_values(*out, *moments):
         return tuple(out)
     # something needs a look
     sizes = [t.numel() for t in exp_avgs]

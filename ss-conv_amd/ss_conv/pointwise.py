@@ -3,6 +3,12 @@ import torch
 
 from ss_conv import _ext
 
+try:
+    from ss_conv import _pointwise as binding  # (csrc/pointwise_torch.cpp)
+except ImportError as e:
+    raise ImportError("ss_conv/_pointwise.so is not built, or not for this torch: run `python "
+                      "ss-conv_amd/build.py --force`") from e
+
 _NAMES = {None: _ext.ACT_NONE, "none": _ext.ACT_NONE, "relu": _ext.ACT_RELU,
           "sigmoid": _ext.ACT_SIGMOID, "tanh": _ext.ACT_TANH, "silu": _ext.ACT_SILU,
           "gelu": _ext.ACT_GELU}
