@@ -174,7 +174,10 @@ __global__ void __launch_bounds__(256)
 // beyond: a lane reads 32 neighbouring bytes of a row of the weights at a step, and rows (16 lanes)
 // and steps are independent, so many loads are in flight.  k is dealt to the lanes as the weights
 // lie in memory, not in the matrix instruction's own order: a sum does not mind as long as x is
-// dealt alike.  Float elements go to float matrix instructions as they are.
+// dealt alike.  Float elements go to float matrix instructions as they are, at 1/16 of the rate of
+// 16-bit ones, so what is multiplied shall not wait for what is loaded: a step ahead 4096 -> 8192 one
+// row 63 -> 54 us, 16 rows 72 -> 57, 20 rows 81 -> 77 (but 64 rows, at half the waves by their registers,
+// 131 -> 140; 16-bit elements gain nothing by it).
 template <typename T> struct FewStep;  // one step: 64 elements along k (16 bits), 32 (float)
 template <> struct FewStep<f16> { static constexpr int kLane = 16; };
 template <> struct FewStep<bf16> { static constexpr int kLane = 16; };
@@ -232,32 +235,51 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmArgs g) {
   f32x4 acc[2 * MT];
 #pragma unroll
   for (int t = 0; t < 2 * MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  int k0 = w * 4 * L;
-#pragma unroll 2
-  for (; k0 + 4 * L <= g.k; k0 += W * 4 * L) {
-    T gv[L], uv[L], xv[MT][L];
-    const int k = k0 + q * L;
-    few_load<T, ALIGNED>(wg + k, L, gv);
-    few_load<T, ALIGNED>(wu + k, L, uv);
+  // A step's elements, `left` of each row's existing; floats in up to 32 rows are loaded one step ahead.
+  struct Step {
+    T gate[L], up[L], x[MT][L];
+  };
+  auto load = [&](Step &s, int k1, int64_t left) {
+    const int k = k1 + q * L;
+    few_load<T, ALIGNED>(wg + k, left - q * L, s.gate);
+    few_load<T, ALIGNED>(wu + k, left - q * L, s.up);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) few_load<T, ALIGNED>(x[t] + k, L, xv[t]);
+    for (int t = 0; t < MT; ++t) few_load<T, ALIGNED>(x[t] + k, left - q * L, s.x[t]);
+  };
+  auto mul = [&](const Step &s) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      few_mul(gv, xv[t], acc[2 * t]);
-      few_mul(uv, xv[t], acc[2 * t + 1]);
+      few_mul(s.gate, s.x[t], acc[2 * t]);
+      few_mul(s.up, s.x[t], acc[2 * t + 1]);
+    }
+  };
+  constexpr int kStep = 4 * L, kNext = W * kStep;
+  constexpr bool kAhead = sizeof(T) == 4 && MT <= 2;
+  int k0 = w * kStep;
+  if constexpr (kAhead) {
+    Step s0, s1;
+    if (k0 + kStep <= g.k) load(s0, k0, kStep);
+    while (k0 + kStep <= g.k) {
+      if (k0 + kNext + kStep <= g.k) load(s1, k0 + kNext, kStep);
+      mul(s0);
+      k0 += kNext;
+      if (k0 + kStep > g.k) break;
+      if (k0 + kNext + kStep <= g.k) load(s0, k0 + kNext, kStep);
+      mul(s1);
+      k0 += kNext;
+    }
+  } else {
+#pragma unroll 2
+    for (; k0 + kStep <= g.k; k0 += kNext) {
+      Step s;
+      load(s, k0, kStep);
+      mul(s);
     }
   }
   if (k0 < g.k) {
-    T gv[L], uv[L], xv[MT][L];
-    const int k = k0 + q * L;
-    few_load<T, ALIGNED>(wg + k, g.k - k, gv);
-    few_load<T, ALIGNED>(wu + k, g.k - k, uv);
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      few_load<T, ALIGNED>(x[t] + k, g.k - k, xv[t]);
-      few_mul(gv, xv[t], acc[2 * t]);
-      few_mul(uv, xv[t], acc[2 * t + 1]);
-    }
+    Step s;
+    load(s, k0, g.k - k0);
+    mul(s);
   }
 #pragma unroll
   for (int t = 0; t < 2 * MT; ++t) lds[w][t][lane] = acc[t];
