@@ -901,3 +901,24 @@ def test_pointwise_checkpoint_hooks_and_accumulation(which):
     for _ in range(2):
         call(*leaves).sum().backward()
     assert all(torch.equal(t.grad, 2 * g) for t, g in zip(leaves, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,h", [(33, 200, 40), (48, 1000, 24), (70, 264, 130), (96, 77, 33),
+                                   (97, 136, 64), (130, 320, 48), (17, 640, 16), (20, 1100, 50)])
+def test_gated_few_rows_in_blocks(m, k, h, dtype):
+    """Blocks of 16, 32, 48 and 64 rows, steps along k that some waves have and others do not."""
+    x, dy = normal((m, k), 1, dtype), normal((m, h), 2, dtype)
+    wg, wu = normal((h, k), 3, dtype, k ** -0.5), normal((h, k), 4, dtype, k ** -0.5)
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    y = gated_linear(*leaves, activation="silu")
+    a, b = [x.detach().double() @ w.detach().double().t() for w in (wg, wu)]
+    f = act64("silu", a)
+    mag_a, mag_b = [x.detach().double().abs() @ w.detach().double().abs().t() for w in (wg, wu)]
+    e_a, e_b = gamma(k) * mag_a, gamma(k) * mag_b
+    e_f = 1.2 * e_a + act_error(a) * (f.abs() + e_a)
+    within(y, f * b, U[dtype] * (f * b).abs() + TINY[dtype] + 2 * (e_f * (b.abs() + e_b) + f.abs() * e_b),
+           "y")
+    assert torch.equal(y.detach(), gated_linear(*[t.detach() for t in leaves]))
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert all(g.shape == t.shape and g.isfinite().all() for g, t in zip(grads, leaves))
