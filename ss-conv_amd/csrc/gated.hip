@@ -14,10 +14,10 @@
 //
 // Many rows: bound by the matrix instructions, at the clock that the power limit leaves (1.75 to
 // 1.95 GHz here): 16384 rows of 2048 -> 8192 in bfloat16, forward with a and b kept 960 to 1080 us
-// (1020 to 1150 TFLOP/s), da and db 320 us (4.9 TB/s), dx 880 us (1250 TFLOP/s), weight gradients 820 us (1340), where
-// torch's library products of these shapes reach 1390 and 1200.  Few rows: bound by the weights'
-// bytes.  Floats: six matrix instructions for one, 57304 rows of 128 -> 512 forward 182 us (bound by
-// storing a, b and y), da and db 113, dx 98, weight gradients 96 + 7.
+// (1020 to 1150 TFLOP/s), da and db 320 us (4.9 TB/s), dx 880 us (1250 TFLOP/s), weight gradients
+// 820 us (1340), where torch's library products of these shapes reach 1390 and 1200.  Few rows: bound
+// by the weights' bytes.  Floats: six matrix instructions for one, 57304 rows of 128 -> 512 forward
+// 182 us (bound by storing a, b and y), da and db 113, dx 98, weight gradients 96 + 7.
 #include "gated_gemm.h"
 
 namespace ssc {

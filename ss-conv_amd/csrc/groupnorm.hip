@@ -32,8 +32,8 @@ namespace {
 
 constexpr int kThreads = 256;
 // Chunks of rows: four workgroups for each of 256 CUs.  More of them pay for finding their cloud and for
-// adding up too often: forward and backward with 2048, 1024 and 512 chunks 50001 x 200 float16 76, 67 and
-// 70 us, 100000 x 64 bfloat16 69, 61 and 57, 600153 x 128 floats 437, 432 and 451.
+// adding up too often: forward and backward with 2048, 1024 and 512 chunks 50001 x 200 float16 76, 67
+// and 70 us, 100000 x 64 bfloat16 69, 61 and 57, 600153 x 128 floats 437, 432 and 451.
 constexpr int kChunksMost = 1024;
 
 struct Norm {
@@ -324,7 +324,8 @@ __device__ __forceinline__ void of_channels(const void *p, int64_t ch, int type,
     // (ch is a multiple of V)
     if (type == SSC_F32) {
 #pragma unroll
-      for (int i = 0; i < V; i += 4) load_floats<float, V < 4 ? V : 4>(static_cast<const float *>(p) + ch + i, out + i);
+      for (int i = 0; i < V; i += 4)
+        load_floats<float, V < 4 ? V : 4>(static_cast<const float *>(p) + ch + i, out + i);
     } else if (type == SSC_F16) {
       load_floats<f16, V>(static_cast<const f16 *>(p) + ch, out);
     } else {
